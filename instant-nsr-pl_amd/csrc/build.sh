@@ -3,7 +3,7 @@
 set -e
 HERE="$(cd "$(dirname "$0")" && pwd)"
 OUT="${1:-$HERE/../nsr_hip}"
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -munsafe-fp-atomics -Wall -Wno-unused-function ${NSR_EXTRA_FLAGS}"
+FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -munsafe-fp-atomics -Wall -Wno-unused-function -Xclang -target-feature -Xclang -packed-fp32-ops ${NSR_EXTRA_FLAGS}"
 mkdir -p "$HERE/obj"
 pids=()
 for f in util hashgrid gridmlp mlp vmlp neus march render fused occupancy step; do
