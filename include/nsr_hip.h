@@ -1039,6 +1039,65 @@ int nsr_masked_loss_backward(const float *pred, const float *target, const uint8
                              int kind, float beta, const float *forward_out, const float *grad_out, float *d_pred,
                              void *stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * AdamW over many tensors of any size, moments in 32 bits or in 8 -- the optimizer of a user's own training system
+ * (torch.optim.AdamW as the reference builds it: systems/utils.py:314-325; clipping and GradScaler as its trainer's
+ * `gradient_clip_val` / `precision: 16` apply them, configs/nerf-blender.yaml:103).
+ *
+ * Descriptors are HOST memory and may be reused when the call returns; the tensors are device memory.  Types: 0 fp32, 1 fp16,
+ * 2 bf16, gradient and parameter alike; arithmetic in fp32, one rounding to nearest at the store.
+ * state_bits 32: exp_avg / exp_avg_sq are float[n].  state_bits 8: blocks of 256 consecutive elements of a tensor; exp_avg and
+ * exp_avg_sq are e4m3 codes [n] of m and of sqrt(v), scales_m / scales_r float[ceil(n / 256)]: value = code * scale.  Codes are
+ * rounded stochastically with bits from a hash of (seed, step, index0 + element); all-zero codes and scales are the zero state.
+ * image (may be NULL): receives the fp16 image of the updated parameters.
+ * An element whose (scaled) gradient is not finite keeps its parameter and moments. */
+typedef struct NsrAdamwTensor {
+    void *params;
+    const void *grad;
+    void *exp_avg, *exp_avg_sq;
+    float *scales_m, *scales_r;
+    nsr_half *image;
+    const float *lr_dev; /* device learning rate that replaces lr, or NULL (only with hyper) */
+    uint64_t n;
+    uint64_t index0;     /* number of the tensor's first element for the random bits: a multiple of 256 */
+    double lr, weight_decay;
+    uint32_t dtype, state_bits;
+} NsrAdamwTensor;
+
+/* One optimizer step over all tensors.  hyper NULL: `step` (1, 2, ...) is this step's number.  hyper (device float[8] written by
+ * nsr_adamw_begin in front of it): step number, gradient factor and the decision to leave the step out are read there. */
+int nsr_adamw_tensors(const NsrAdamwTensor *tensors, uint32_t n_tensors, double beta1, double beta2, double eps, int32_t step,
+                      const float *hyper, double grad_unscale, uint32_t seed, void *stream);
+
+/* Sums of squares of all gradients (only grad, n and dtype of a descriptor are read), in 64 bits: partials[*n_partials], at most
+ * nsr_grad_squares_capacity of them.  n_partials is HOST memory, known when the call returns. */
+uint32_t nsr_grad_squares_capacity(const NsrAdamwTensor *tensors, uint32_t n_tensors);
+int nsr_grad_squares(const NsrAdamwTensor *tensors, uint32_t n_tensors, double *partials, uint32_t capacity,
+                     uint32_t *n_partials, void *stream);
+
+/* Opens an optimizer step whose count lives on the device (int32[1]).  partials (may be NULL): norm = sqrt(their sum), gradients
+ * are scaled by min(1, max_norm / (norm + 1e-6)) and the step is left out when the norm is not finite.  grad_scale / found_inf
+ * (device float[1], may be NULL): GradScaler's -- gradients are divided by the one (the norm is that of the divided ones), the
+ * step is left out when the other is not zero.  A step that is left out does not count.
+ * hyper[8]: {gradient factor, 1 / (1 - beta1^t), 1 / sqrt(1 - beta2^t), left out (int bits), t (int bits), norm, -, -}. */
+int nsr_adamw_begin(int32_t *step, float *hyper, double beta1, double beta2, const double *partials, uint32_t n_partials,
+                    double max_norm, const float *grad_scale, const float *found_inf, void *stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Layer norm over the last axis, for networks beside the fused 64-wide ones (the reference's VanillaMLP takes any torch layer:
+ * models/network_utils.py:100-139).  Types as above; weight and bias (both may be NULL) are fp32 or of the input's type.
+ * x and dy have a row stride in elements, y and dx are contiguous.  Statistics and sums in fp32.
+ * ------------------------------------------------------------------------------------------------ */
+/* y = (x - mean) * rstd * weight + bias; mean / rstd (float[rows], both or neither) are kept for the backward pass */
+int nsr_layer_norm_forward(const void *x, uint64_t x_stride, const void *weight, const void *bias, void *y, float *mean,
+                           float *rstd, uint64_t rows, uint32_t width, uint32_t dtype, uint32_t affine_dtype, float eps,
+                           void *stream);
+uint64_t nsr_layer_norm_backward_workspace_floats(uint64_t rows, uint32_t width);
+/* dx, dweight, dbias (each may be NULL) are overwritten; workspace only for dweight / dbias.  Same bits for the same inputs. */
+int nsr_layer_norm_backward(const void *dy, uint64_t dy_stride, const void *x, uint64_t x_stride, const void *weight,
+                            const float *mean, const float *rstd, void *dx, void *dweight, void *dbias, float *workspace,
+                            uint64_t rows, uint32_t width, uint32_t dtype, uint32_t affine_dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,345 @@
+"""AdamW over any number of tensors for a user's own training system (the reference's ``parse_optimizer`` builds
+``torch.optim.AdamW``: systems/utils.py:314-325; the trainers of this package own their optimizers and do not need it)."""
+import ctypes
+import math
+
+import numpy as np
+import torch
+
+from nsr_hip import NsrAdamwTensor, NsrError, check, device_guard, lib, ptr, stream_ptr
+from nsr_hip.ops import DTYPE_CODES, timed
+
+F32, F8 = torch.float32, torch.float8_e4m3fn
+BLOCK = 256  # elements under one scale of the 8-bit moments (csrc/optim.hip); every tensor's moments start at a multiple of it
+
+
+def _is_dense(t):
+    """``t``'s elements fill one span of memory, in whatever order of its axes"""
+    if t.is_contiguous():
+        return True
+    order = sorted(range(t.dim()), key=lambda d: (-t.stride(d), -t.shape[d]))
+    return t.permute(order).is_contiguous()
+
+
+class AdamW(torch.optim.Optimizer):
+    """``torch.optim.AdamW`` (decoupled weight decay, bias correction) with all tensors updated in one launch per 36 of them.
+
+    ``state_bits=8``: moments in 8 bits with one float32 scale per 256 elements and moment (16.1 instead of 28 bytes of memory
+    traffic per float32 parameter and step, 2.06 instead of 8 bytes of state).  They are rounded stochastically, with random bits
+    made from (``rounding_seed``, step, element): the same run gives the same bits.  Tensors with fewer than ``min_8bit_size``
+    elements keep 32-bit moments.
+
+    ``max_grad_norm``: gradients are scaled by min(1, max_grad_norm / (norm + 1e-6)) with the norm over the gradients of all
+    tensors; a step whose norm is not finite is left out whole.  ``grad_norm`` holds the last step's norm (a 0-dim GPU tensor that
+    the next step overwrites).  Nothing is read back to the host.
+
+    ``capturable=True``: the step count lives on the device and ``step`` may be captured into a graph; the learning rate that a
+    replay uses is a group's ``lr`` tensor (0-dim or one element, float32, on the GPU) or, if it is a number, the captured one.
+
+    ``modules``: ``tinycudann`` modules whose ``params`` are among the parameters: the fp16 image that their kernels read is
+    written in the same pass (otherwise they cast ``params`` again in every forward pass).
+
+    Parameters are float32, float16 or bfloat16 (arithmetic and 32-bit moments in float32), dense and on one GPU; ``betas`` and
+    ``eps`` are the same for all groups, ``lr`` and ``weight_decay`` are the group's.  Tensors whose ``grad`` is None are left
+    as they are; the step count is one for all tensors.  An element whose gradient is not finite keeps its value and moments.
+    Works with ``torch.amp.GradScaler`` without a synchronisation of its own: gradients are unscaled in the pass, a step with a
+    non-finite one is left out.  32-bit state dicts can be exchanged with ``torch.optim.AdamW``'s."""
+
+    _step_supports_amp_scaling = True
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, *, state_bits=32, min_8bit_size=4096,
+                 max_grad_norm=None, capturable=False, modules=(), rounding_seed=0):
+        if state_bits not in (8, 32):
+            raise ValueError(f"AdamW: state_bits is 8 or 32, got {state_bits}")
+        if max_grad_norm is not None and not 0.0 < float(max_grad_norm) < math.inf:
+            raise ValueError(f"AdamW: max_grad_norm {max_grad_norm}")
+        if not 0 <= int(rounding_seed) < 1 << 32:
+            raise ValueError(f"AdamW: rounding_seed is a 32-bit number, got {rounding_seed}")
+        self._built = False
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+        self.state_bits, self.min_8bit_size = int(state_bits), int(min_8bit_size)
+        self.max_grad_norm = None if max_grad_norm is None else float(max_grad_norm)
+        self.capturable, self.rounding_seed = bool(capturable), int(rounding_seed)
+        self._step, self._step_dev, self._hyper, self._partials = 0, None, None, None
+        self._lay_out()
+        self._images = self._image_modules(modules)
+        self._shared_hyperparameters()
+        for g in self.param_groups:
+            self._learning_rate(g)
+        if self.capturable or self.max_grad_norm is not None:
+            self._device_step()
+        self._built = True
+
+    # ---- construction --------------------------------------------------------------------------------------------------------
+    def _lay_out(self):
+        """every tensor's place in the flat moments, its descriptor, and ``self.state`` as views of them"""
+        items = [(p, i) for i, g in enumerate(self.param_groups) for p in g["params"]]
+        spans = []
+        for p, _ in items:
+            if not p.is_cuda:
+                raise NsrError("AdamW: parameters live on the GPU (there is no CPU path in the product library)")
+            if p.dtype not in DTYPE_CODES:
+                raise NsrError(f"AdamW: float32/float16/bfloat16 parameters, got {p.dtype}")
+            if p.device != items[0][0].device:
+                raise NsrError(f"AdamW: parameters on {p.device} and {items[0][0].device}")
+            if not _is_dense(p):
+                raise NsrError(f"AdamW: a parameter of shape {tuple(p.shape)} with strides {p.stride()} is not dense")
+            if p.numel():
+                spans.append((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()))
+        spans.sort()
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("AdamW: two parameters share memory")
+        self.device = items[0][0].device
+        self._ps = [p for p, _ in items]
+        self._group_of = [i for _, i in items]
+        self._dense = [p.is_contiguous() for p in self._ps]
+        self._bits = [8 if self.state_bits == 8 and p.numel() >= self.min_8bit_size else 32 for p in self._ps]
+        self._at, total = [], {8: 0, 32: 0}
+        for p, bits in zip(self._ps, self._bits):
+            self._at.append(total[bits])
+            total[bits] += -(-p.numel() // BLOCK) * BLOCK
+        new = lambda n, dtype: torch.zeros(n, dtype=torch.uint8 if dtype is F8 else dtype, device=self.device).view(dtype)  # noqa: E731
+        # flat moments: tensor i has [at, at + numel) of the set of its width, zeros behind it up to the next multiple of BLOCK
+        self.flat32 = {k: new(total[32], F32) for k in ("exp_avg", "exp_avg_sq")} if total[32] else {}
+        self.flat8 = {}
+        if total[8]:
+            self.flat8 = {k: new(total[8], F8) for k in ("exp_avg", "exp_avg_rms")}
+            self.flat8["scales"] = torch.zeros(2, total[8] // BLOCK, dtype=F32, device=self.device)
+        n = len(self._ps)
+        self._desc = (NsrAdamwTensor * n)()
+        self._fields = np.frombuffer(self._desc, dtype=np.dtype(NsrAdamwTensor))
+        f = self._fields
+        f["n"] = [p.numel() for p in self._ps]
+        f["params"] = [p.data_ptr() for p in self._ps]
+        f["dtype"] = [DTYPE_CODES[p.dtype] for p in self._ps]
+        f["state_bits"] = self._bits
+        f["index0"] = self._at
+        for i, (at, bits) in enumerate(zip(self._at, self._bits)):
+            if bits == 8:
+                d = self._desc[i]
+                d.exp_avg, d.exp_avg_sq = self.flat8["exp_avg"].data_ptr() + at, self.flat8["exp_avg_rms"].data_ptr() + at
+                d.scales_m = self.flat8["scales"].data_ptr() + 4 * (at // BLOCK)
+                d.scales_r = d.scales_m + 4 * self.flat8["scales"].shape[1]
+            elif f["n"][i]:
+                d = self._desc[i]
+                d.exp_avg, d.exp_avg_sq = (self.flat32[k].data_ptr() + 4 * at for k in ("exp_avg", "exp_avg_sq"))
+        self._bind_state()
+
+    def _bind_state(self):
+        for p, at, bits in zip(self._ps, self._at, self._bits):
+            flat, n = self.flat8 if bits == 8 else self.flat32, p.numel()
+            if not n:
+                continue
+            s = {k: t[at:at + n].as_strided(p.shape, p.stride()) for k, t in flat.items() if k != "scales"}
+            if bits == 8:
+                s["scales"] = flat["scales"][:, at // BLOCK:-(-(at + n) // BLOCK)]
+            self.state[p] = s
+
+    def _image_modules(self, modules):
+        place = {id(p): i for i, p in enumerate(self._ps)}
+        found = []
+        for m in modules:
+            if m.params.numel() == 0:
+                continue
+            i = place.get(id(m.params))
+            if i is None or m.params.dtype != F32:
+                raise ValueError("AdamW: `modules` are tinycudann modules whose float32 `params` are among the parameters")
+            image = torch.empty_like(m.params, dtype=torch.float16)
+            self._desc[i].image = image.data_ptr()
+            found.append((m, i, image))
+        return found
+
+    def add_param_group(self, param_group):
+        if getattr(self, "_built", False):
+            raise NotImplementedError("AdamW: the parameters are fixed at construction (their moments lie in flat buffers)")
+        super().add_param_group(param_group)
+
+    def __getstate__(self):
+        raise NotImplementedError("AdamW: copy an optimizer through state_dict() / load_state_dict()")
+
+    # ---- hyperparameters -----------------------------------------------------------------------------------------------------
+    def _shared_hyperparameters(self):
+        g0 = self.param_groups[0]
+        (b1, b2), eps = g0["betas"], g0["eps"]
+        for g in self.param_groups:
+            if tuple(g["betas"]) != (b1, b2) or g["eps"] != eps:
+                raise NotImplementedError("AdamW: betas and eps are the same for all groups")
+            if g.get("amsgrad") or g.get("maximize"):  # (a state dict of torch.optim.AdamW's)
+                raise NotImplementedError("AdamW: neither amsgrad nor maximize")
+            if not g["weight_decay"] >= 0.0:
+                raise ValueError(f"AdamW: weight_decay {g['weight_decay']}")
+        if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0):
+            raise ValueError(f"AdamW: betas {(b1, b2)}, eps {eps}")
+        return b1, b2, eps
+
+    def _learning_rate(self, group):
+        """(number, device pointer) of a group's learning rate"""
+        lr = group["lr"]
+        if isinstance(lr, torch.Tensor):
+            if lr.numel() != 1 or lr.dtype != F32:
+                raise ValueError(f"AdamW: a learning rate tensor has one float32 element, got {tuple(lr.shape)} {lr.dtype}")
+            if self.capturable:
+                if lr.device != self.device:
+                    raise ValueError(f"AdamW: the learning rate of a capturable optimizer is on {self.device}, got {lr.device}")
+                return 0.0, lr.data_ptr()
+            lr = float(lr)
+        if not lr >= 0.0:
+            raise ValueError(f"AdamW: lr {lr}")
+        return float(lr), None
+
+    # ---- step count ----------------------------------------------------------------------------------------------------------
+    def _device_step(self):
+        if self._step_dev is None:
+            self._step_dev = torch.full((1,), self._step, dtype=torch.int32, device=self.device)
+            self._hyper = torch.zeros(8, dtype=F32, device=self.device)
+        return self._step_dev, self._hyper
+
+    def taken_steps(self):
+        """optimizer steps taken, those left out not among them (synchronises where the count lives on the device)"""
+        return self._step if self._step_dev is None else int(self._step_dev.item())
+
+    def set_step(self, count):
+        """the next step is number ``count`` + 1"""
+        self._step = int(count)
+        if self._step_dev is not None:
+            self._step_dev.fill_(self._step)
+
+    @property
+    def grad_norm(self):
+        """norm of the last step's gradients before clipping (None without ``max_grad_norm``)"""
+        return self._hyper[5] if self.max_grad_norm is not None else None
+
+    # ---- one step ------------------------------------------------------------------------------------------------------------
+    def _gather(self):
+        """this step's addresses in the descriptors; (host array, count, live parameters, tensors to keep until the launch)"""
+        f, live, keep = self._fields, [], []
+        grads, params = [], []
+        for i, p in enumerate(self._ps):
+            g = p.grad
+            if g is None:
+                continue
+            if not g.is_contiguous() or not self._dense[i]:
+                if g.is_sparse:
+                    raise NsrError("AdamW: sparse gradients are not supported")
+                if g.stride() != p.stride():
+                    keep.append(torch.empty_strided(p.shape, p.stride(), dtype=p.dtype, device=p.device).copy_(g))
+                    g = keep[-1]
+            live.append(i)
+            grads.append(g.data_ptr())
+            params.append(p.data_ptr())
+        if len(live) == len(self._ps):
+            f["grad"], old = grads, f["params"].copy()
+            f["params"] = params
+            if not np.array_equal(f["params"], old):
+                self._check_moved()
+            return self._desc, len(live), self._ps, keep
+        for i, g, a in zip(live, grads, params):
+            f["grad"][i] = g
+            if f["params"][i] != a:
+                f["params"][i] = a
+                self._check_moved()
+        some = f[live]  # (a copy)
+        return some.ctypes.data, len(live), [self._ps[i] for i in live], keep + [some]
+
+    def _check_moved(self):
+        """parameters whose memory was replaced (``p.data = ...``) still have the layout that the moments were made for"""
+        for i, p in enumerate(self._ps):
+            if p.numel() != self._fields["n"][i] or DTYPE_CODES.get(p.dtype) != self._fields["dtype"][i] or \
+                    p.device != self.device or not _is_dense(p) or (p.numel() and p.stride() != self._stride(i)):
+                raise NsrError(f"AdamW: parameter {i} changed its shape, type, strides or device since construction")
+
+    def _stride(self, i):
+        return next(iter(self.state[self._ps[i]].values())).stride()
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        b1, b2, eps = self._shared_hyperparameters()
+        scale, found = getattr(self, "grad_scale", None), getattr(self, "found_inf", None)
+        if self._step_dev is None and (scale is not None or found is not None):
+            self._device_step()  # (a step may be left out: only the device knows the count)
+        if not self.capturable and torch.cuda.is_current_stream_capturing():
+            raise NsrError("AdamW: only an optimizer with capturable=True can step inside a graph capture")
+        f = self._fields
+        rates = [self._learning_rate(g) for g in self.param_groups]
+        if len(rates) == 1:
+            f["lr"], f["lr_dev"] = rates[0][0], rates[0][1] or 0
+            f["weight_decay"] = self.param_groups[0]["weight_decay"]
+        else:
+            f["lr"] = [rates[i][0] for i in self._group_of]
+            f["lr_dev"] = [rates[i][1] or 0 for i in self._group_of]
+            f["weight_decay"] = [self.param_groups[i]["weight_decay"] for i in self._group_of]
+        desc, n, live, keep = self._gather()
+        if n == 0:
+            return loss
+        with device_guard(self.device), timed("adamw_step", n):
+            for m, i, image in self._images:
+                p = m.params
+                if m._shadow is not image or not m._shadow_trusted or m._shadow_key != (p.data_ptr(), p._version, p.device):
+                    image.copy_(p)  # first step, or the parameters were written from outside
+            s = stream_ptr()
+            if self._step_dev is None:
+                self._step += 1
+                step, hyper = self._step, None
+            else:
+                self._begin(desc, n, b1, b2, scale, found, s)
+                step, hyper = 0, ptr(self._hyper)
+            check(lib.nsr_adamw_tensors(desc, n, b1, b2, eps, step, hyper, 1.0, self.rounding_seed, s), "nsr_adamw_tensors")
+        torch.autograd.graph.increment_version(live)
+        for m, i, image in self._images:
+            m.adopt_shadow(image)
+        return loss
+
+    def _begin(self, desc, n, b1, b2, scale, found, stream):
+        count, partials, clip = 0, None, 0.0
+        if self.max_grad_norm is not None:
+            if self._partials is None:
+                room = lib.nsr_grad_squares_capacity(self._desc, len(self._ps))
+                self._partials = torch.empty(room, dtype=torch.float64, device=self.device)
+            got = ctypes.c_uint32()
+            check(lib.nsr_grad_squares(desc, n, self._partials.data_ptr(), self._partials.numel(), ctypes.byref(got), stream),
+                  "nsr_grad_squares")
+            count, partials, clip = got.value, self._partials.data_ptr(), self.max_grad_norm
+        for t in (scale, found):
+            if t is not None and (t.dtype != F32 or t.device != self.device or t.numel() != 1):
+                raise NsrError("AdamW: grad_scale and found_inf are one float32 element on the parameters' device")
+        check(lib.nsr_adamw_begin(ptr(self._step_dev), ptr(self._hyper), b1, b2, partials, count, clip,
+                                  None if scale is None else scale.data_ptr(), None if found is None else found.data_ptr(),
+                                  stream), "nsr_adamw_begin")
+
+    # ---- checkpoints ---------------------------------------------------------------------------------------------------------
+    def state_dict(self):
+        """torch's layout; every tensor's state holds the common ``step`` as well"""
+        sd, step = super().state_dict(), float(self.taken_steps())
+        sd["state"] = {k: {"step": torch.tensor(step), **v} for k, v in sd["state"].items()}
+        return sd
+
+    def load_state_dict(self, state_dict):
+        """state of an optimizer with the same tensors and the same ``state_bits`` for each of them (the moments keep their own
+        types, unlike in torch, which casts them to the parameter's)"""
+        saved, steps = state_dict["state"], set()
+        for i, p in enumerate(self._ps):
+            if i not in saved or not p.numel():
+                continue
+            for k, t in self.state[p].items():
+                v = saved[i].get(k)
+                if v is None or v.dtype != t.dtype or v.shape != t.shape:
+                    raise ValueError(f"AdamW.load_state_dict: tensor {i} needs {k} {tuple(t.shape)} {t.dtype}, the state has "
+                                     f"{None if v is None else (tuple(v.shape), v.dtype)}")
+            steps.add(float(saved[i]["step"]))
+        if len(steps) > 1:
+            raise ValueError(f"AdamW.load_state_dict: the tensors' step counts differ: {sorted(steps)}")
+        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
+        self._bind_state()
+        for i, p in enumerate(self._ps):
+            for k, t in self.state.get(p, {}).items():
+                if i not in saved:
+                    (t.view(torch.uint8) if t.dtype is F8 else t).zero_()
+                elif t.dtype is F8:
+                    t.view(torch.uint8).copy_(saved[i][k].to(self.device).view(torch.uint8))
+                else:
+                    t.copy_(saved[i][k])
+        self.set_step(int(steps.pop()) if steps else 0)

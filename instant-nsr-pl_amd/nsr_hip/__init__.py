@@ -83,6 +83,14 @@ class NsrAdamSegment(ctypes.Structure):
                 ("exp_avg_sq", ctypes.c_void_p), ("n", ctypes.c_uint64), ("lr", ctypes.c_float)]
 
 
+class NsrAdamwTensor(ctypes.Structure):
+    """include/nsr_hip.h: one tensor of an AdamW step over many (host memory)"""
+    _fields_ = [(k, ctypes.c_void_p) for k in ("params", "grad", "exp_avg", "exp_avg_sq", "scales_m", "scales_r", "image",
+                                               "lr_dev")] + \
+        [("n", ctypes.c_uint64), ("index0", ctypes.c_uint64), ("lr", ctypes.c_double), ("weight_decay", ctypes.c_double),
+         ("dtype", ctypes.c_uint32), ("state_bits", ctypes.c_uint32)]
+
+
 class NsrVmlpDesc(ctypes.Structure):
     _fields_ = [("n_in", ctypes.c_uint32), ("in_pad", ctypes.c_uint32), ("n_out", ctypes.c_uint32),
                 ("n_hidden", ctypes.c_uint32), ("activation", ctypes.c_uint32)]
@@ -254,6 +262,13 @@ SIGNATURES = {
     "nsr_vmlp_fold": [_VD, _P, _U, _P, _P],
     "nsr_vmlp_unfold_gradient": [_VD, _P, _U, _P, _I, _P],
     "nsr_adamw_multi": [_P, _U, _F, _F, _F, _F, _F, _F, _I, _P, _P, _P],
+    "nsr_adamw_tensors": [_P, _U, _D, _D, _D, ctypes.c_int32, _P, _D, _U, _P],
+    "nsr_grad_squares_capacity": [_P, _U],
+    "nsr_grad_squares": [_P, _U, _P, _U, ctypes.POINTER(ctypes.c_uint32), _P],
+    "nsr_adamw_begin": [_P, _P, _D, _D, _P, _U, _D, _P, _P, _P],
+    "nsr_layer_norm_forward": [_P, _U64, _P, _P, _P, _P, _P, _U64, _U, _U, _U, _F, _P],
+    "nsr_layer_norm_backward_workspace_floats": [_U64, _U],
+    "nsr_layer_norm_backward": [_P, _U64, _P, _U64, _P, _P, _P, _P, _P, _P, _P, _U64, _U, _U, _U, _P],
     "nsr_neus_inv_s": [_P, _P, _P],
     "nsr_neus_occupancy_values": [_P, _P, _F, _P, _U, _P, _P],
     "nsr_occupancy_update_values": [_P, _F, _F, _P, _P, _P, _P, _P, _U, _U, _P, _P],
@@ -273,7 +288,8 @@ SIGNATURES = {
     "nsr_neus_shade_backward": [_P, _P, _P, _P, _P, _P, _P, _F, _P, _F, _F, _P, _P, _U, _P, _F, _F, _P, _P, _P, _U, _P,
                                 _P, _U, _P, _P],
 }
-_RESTYPES = {"nsr_last_error": ctypes.c_char_p, "nsr_ray_march_rays_per_wave": ctypes.c_uint32, "nsr_nerf_helper_stream": ctypes.c_void_p, "nsr_hashgrid_owner_large_from": ctypes.c_uint32, "nsr_hashgrid_owner_tune": ctypes.c_float, "nsr_mlp_wgrad_max_blocks": ctypes.c_uint32, "nsr_masked_loss_out_floats": ctypes.c_uint32,
+_RESTYPES = {"nsr_grad_squares_capacity": ctypes.c_uint32, "nsr_layer_norm_backward_workspace_floats": ctypes.c_uint64,
+             "nsr_last_error": ctypes.c_char_p, "nsr_ray_march_rays_per_wave": ctypes.c_uint32, "nsr_nerf_helper_stream": ctypes.c_void_p, "nsr_hashgrid_owner_large_from": ctypes.c_uint32, "nsr_hashgrid_owner_tune": ctypes.c_float, "nsr_mlp_wgrad_max_blocks": ctypes.c_uint32, "nsr_masked_loss_out_floats": ctypes.c_uint32,
              "nsr_composite_l1_partials_floats": ctypes.c_uint64,
              "nsr_grid_mlp_backward_workspace_floats": ctypes.c_uint64, "nsr_mlp_backward_workspace_floats": ctypes.c_uint64,
              "nsr_vmlp_blob_floats": ctypes.c_uint64, "nsr_vmlp_backward_workspace_floats": ctypes.c_uint64,

@@ -826,3 +826,123 @@ def adam_tick(step_dev, hyper_dev, base_lr, beta1, beta2, gamma, milestones):
     with device_guard(step_dev.device):
         check(lib.nsr_adam_tick(ptr(step_dev), ptr(hyper_dev), float(base_lr), float(beta1), float(beta2), float(gamma),
                                 ms[0], ms[1], ms[2], stream_ptr()), "nsr_adam_tick")
+
+
+# ------------------------------------------------------------------------------------------------
+# layer norm
+# ------------------------------------------------------------------------------------------------
+BF16 = torch.bfloat16
+DTYPE_CODES = {F32: 0, F16: 1, BF16: 2}  # of the C ABI's training operators
+
+
+def _rows(t, width):
+    """(tensor, rows, row stride in elements): ``t`` itself where its last axis is dense and its rows lie evenly apart, else a
+    contiguous copy"""
+    if t.is_contiguous():
+        return t, t.numel() // width, width
+    if t.dim() == 2 and (t.stride(1) == 1 or width == 1) and t.stride(0) >= width:
+        return t, t.shape[0], t.stride(0)
+    return t.contiguous(), t.numel() // width, width
+
+
+def _ln_check(x, weight, bias):
+    if x.dtype not in DTYPE_CODES:
+        raise NsrError(f"layer_norm: expected a float32/float16/bfloat16 tensor, got {x.dtype}")
+    if not x.is_cuda:
+        raise NsrError("nsr_hip ops need GPU tensors (there is no CPU path in the product library)")
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError(f"layer_norm: no last axis to normalise in shape {tuple(x.shape)}")
+    affine = None
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        if t.dim() != 1 or t.shape[0] != x.shape[-1]:
+            raise ValueError(f"layer_norm: {name} has shape {tuple(t.shape)}, expected ({x.shape[-1]},)")
+        if t.dtype != F32 and t.dtype != x.dtype or affine not in (None, t.dtype):
+            raise NsrError(f"layer_norm: weight and bias are both float32 or both {x.dtype}, got {t.dtype}")
+        if t.device != x.device:
+            raise NsrError(f"layer_norm: {name} is on {t.device}, the input on {x.device}")
+        affine = t.dtype
+    return x.dtype if affine is None else affine
+
+
+def _layer_norm(x, weight, bias, eps, want_stats):
+    affine = _ln_check(x, weight, bias)
+    width = x.shape[-1]
+    xr, rows, stride = _rows(x, width)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean = rstd = None
+    if want_stats:
+        stats = torch.empty((2,) + x.shape[:-1], dtype=F32, device=x.device)
+        mean, rstd = stats[0], stats[1]
+    weight = weight if weight is None else weight.contiguous()
+    bias = bias if bias is None else bias.contiguous()
+    with device_guard(x.device), _timed("layer_norm_forward", rows):
+        check(lib.nsr_layer_norm_forward(xr.data_ptr(), stride, ptr(weight), ptr(bias), y.data_ptr(), ptr(mean), ptr(rstd), rows,
+                                         width, DTYPE_CODES[x.dtype], DTYPE_CODES[affine], float(eps), stream_ptr()),
+              "nsr_layer_norm_forward")
+    return y, mean, rstd
+
+
+def layer_norm_forward(x, weight=None, bias=None, eps=1e-5):
+    """``(y, mean, rstd)``: ``x`` [..., width] normalised over its last axis, times ``weight`` plus ``bias`` ([width], float32 or
+    ``x``'s type; either may be None), and the rows' statistics in float32 (``x.shape[:-1]``) for ``layer_norm_backward``"""
+    return _layer_norm(x, weight, bias, eps, True)
+
+
+def layer_norm_backward(dy, x, weight, mean, rstd, want_dx=True, want_dweight=True, want_dbias=True, affine_dtype=None):
+    """``(dx, dweight, dbias)`` of ``layer_norm_forward`` (None where not wanted).  ``dweight`` / ``dbias`` have ``weight``'s type
+    (``affine_dtype``, by default ``x``'s, without one); sums over the rows are in float32 and the same for the same inputs."""
+    affine = _ln_check(x, weight, None)
+    if weight is None and affine_dtype is not None:
+        if affine_dtype not in (F32, x.dtype):
+            raise NsrError(f"layer_norm: affine gradients are float32 or {x.dtype}, got {affine_dtype}")
+        affine = affine_dtype
+    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
+        raise ValueError(f"layer_norm_backward: dy is {tuple(dy.shape)} {dy.dtype} on {dy.device}, the input "
+                         f"{tuple(x.shape)} {x.dtype} on {x.device}")
+    for t in (mean, rstd):
+        if t.shape != x.shape[:-1] and t.numel() * x.shape[-1] != x.numel() or t.dtype != F32 or t.device != x.device:
+            raise ValueError("layer_norm_backward: mean and rstd are the float32 rows' statistics of layer_norm_forward")
+    width, dev = x.shape[-1], x.device
+    xr, rows, stride = _rows(x, width)
+    dr, _, dstride = _rows(dy, width)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_dx else None
+    dweight = torch.empty(width, dtype=affine, device=dev) if want_dweight else None
+    dbias = torch.empty(width, dtype=affine, device=dev) if want_dbias else None
+    ws = None
+    if want_dweight or want_dbias:
+        ws = torch.empty(lib.nsr_layer_norm_backward_workspace_floats(rows, width), dtype=F32, device=dev)
+    weight = weight if weight is None else weight.contiguous()
+    mean, rstd = mean.contiguous(), rstd.contiguous()
+    with device_guard(dev), _timed("layer_norm_backward", rows):
+        check(lib.nsr_layer_norm_backward(dr.data_ptr(), dstride, xr.data_ptr(), stride, ptr(weight), ptr(mean), ptr(rstd), ptr(dx),
+                                          ptr(dweight), ptr(dbias), ptr(ws), rows, width, DTYPE_CODES[x.dtype],
+                                          DTYPE_CODES[affine], stream_ptr()), "nsr_layer_norm_backward")
+    return dx, dweight, dbias
+
+
+class _LayerNorm(Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = _layer_norm(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, mean, rstd = ctx.saved_tensors
+        want = ctx.needs_input_grad
+        dx, dw, db = layer_norm_backward(dy, x, weight, mean, rstd, want[0], want[1], want[2], affine_dtype=ctx.bias_dtype)
+        return dx, dw, db, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """layer norm over the last axis, differentiable once (a second differentiation raises); types and shapes as in
+    ``layer_norm_forward``.  Nothing but ``y`` is written where no gradient is wanted."""
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
+                                    (bias is not None and bias.requires_grad)):
+        return _LayerNorm.apply(x, weight, bias, float(eps))
+    return _layer_norm(x, weight, bias, eps, False)[0]
