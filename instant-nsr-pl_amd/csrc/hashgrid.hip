@@ -289,7 +289,8 @@ __device__ __forceinline__ void blend8(const Cell &c, const float (&v)[8][F], __
         yo[0] = __float2half_rn(acc[0]);
     } else {
 #pragma unroll
-        for (int f = 0; f < F; f += 2) *reinterpret_cast<__half2 *>(yo + f) = __floats2half2_rn(acc[f], acc[f + 1]);
+        for (int f = 0; f < F; f += 2)  // (the same bits as the plain encode: fp32 sum, then fp16)
+            *reinterpret_cast<__half2 *>(yo + f) = __floats2half2_rn(nsr_rounded(acc[f]), nsr_rounded(acc[f + 1]));
     }
 }
 

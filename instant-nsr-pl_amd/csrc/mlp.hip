@@ -501,7 +501,7 @@ k_mlp_dgrad_pair(const float *__restrict__ d_rgb /* [n,3] */, const float *__res
 #pragma unroll
             for (int r = 0; r < 4; ++r) d_o[r] = dfeat[r] * grad_scale;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) gout_d[t32_off(s, 4 * g + r, 16)] = __float2half_rn(d_o[r]);
+            for (int r = 0; r < 4; ++r) gout_d[t32_off(s, 4 * g + r, 16)] = __float2half_rn(nsr_rounded(d_o[r]));
         } else {
             d_o = f32x4{0.f, 0.f, 0.f, 0.f};
         }

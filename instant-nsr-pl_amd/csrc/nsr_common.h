@@ -65,6 +65,15 @@ __device__ __forceinline__ uint32_t live_count(uint32_t n, const int32_t *__rest
     return v < 0 ? 0u : ((uint32_t)v < n ? (uint32_t)v : n);
 }
 
+// An fp32 result that is rounded to fp16 as a second rounding.  Without it the compiler may fold the conversion into the
+// multiplication or fma in front of it (v_fma_mixlo_f16 rounds once), which differs in the last bit from kernels of the same
+// formula whose code happens not to fold.
+__device__ __forceinline__ float nsr_rounded(float v)
+{
+    asm("" : "+v"(v));
+    return v;
+}
+
 // fp32 -> bf16, round to nearest even (NaN stays NaN); two values packed low | high << 16
 __device__ __forceinline__ uint32_t nsr_to_bf16(float f)
 {
