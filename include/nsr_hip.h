@@ -1092,7 +1092,7 @@ int nsr_adamw_begin(int32_t *step, float *hyper, double beta1, double beta2, con
 int nsr_layer_norm_forward(const void *x, uint64_t x_stride, const void *weight, const void *bias, void *y, float *mean,
                            float *rstd, uint64_t rows, uint32_t width, uint32_t dtype, uint32_t affine_dtype, float eps,
                            void *stream);
-uint64_t nsr_layer_norm_backward_workspace_floats(uint64_t rows, uint32_t width);
+uint64_t nsr_layer_norm_backward_workspace_floats(uint64_t rows, uint32_t width, uint32_t dtype);
 /* dx, dweight, dbias (each may be NULL) are overwritten; workspace only for dweight / dbias.  Same bits for the same inputs. */
 int nsr_layer_norm_backward(const void *dy, uint64_t dy_stride, const void *x, uint64_t x_stride, const void *weight,
                             const float *mean, const float *rstd, void *dx, void *dweight, void *dbias, float *workspace,

@@ -267,7 +267,7 @@ SIGNATURES = {
     "nsr_grad_squares": [_P, _U, _P, _U, ctypes.POINTER(ctypes.c_uint32), _P],
     "nsr_adamw_begin": [_P, _P, _D, _D, _P, _U, _D, _P, _P, _P],
     "nsr_layer_norm_forward": [_P, _U64, _P, _P, _P, _P, _P, _U64, _U, _U, _U, _F, _P],
-    "nsr_layer_norm_backward_workspace_floats": [_U64, _U],
+    "nsr_layer_norm_backward_workspace_floats": [_U64, _U, _U],
     "nsr_layer_norm_backward": [_P, _U64, _P, _U64, _P, _P, _P, _P, _P, _P, _P, _U64, _U, _U, _U, _P],
     "nsr_neus_inv_s": [_P, _P, _P],
     "nsr_neus_occupancy_values": [_P, _P, _F, _P, _U, _P, _P],

@@ -912,7 +912,7 @@ def layer_norm_backward(dy, x, weight, mean, rstd, want_dx=True, want_dweight=Tr
     dbias = torch.empty(width, dtype=affine, device=dev) if want_dbias else None
     ws = None
     if want_dweight or want_dbias:
-        ws = torch.empty(lib.nsr_layer_norm_backward_workspace_floats(rows, width), dtype=F32, device=dev)
+        ws = torch.empty(lib.nsr_layer_norm_backward_workspace_floats(rows, width, DTYPE_CODES[x.dtype]), dtype=F32, device=dev)
     weight = weight if weight is None else weight.contiguous()
     mean, rstd = mean.contiguous(), rstd.contiguous()
     with device_guard(dev), _timed("layer_norm_backward", rows):
