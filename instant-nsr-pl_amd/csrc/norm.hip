@@ -13,6 +13,8 @@
 // order (no atomics: the same bits for the same inputs).
 #include "elem.h"
 
+#include <type_traits>
+
 namespace {
 
 constexpr uint32_t CUS = 256;
@@ -425,6 +427,7 @@ k_ln_backward_finish(const float *__restrict__ part, uint32_t n, uint32_t width,
     const uint64_t col = (uint64_t)blockIdx.x * 16 + threadIdx.x % 16;
     float acc = 0.f;
     if (col < 2ull * width)
+#pragma unroll 8
         for (uint32_t s = threadIdx.x / 16; s < n; s += 64) acc += part[s * 2ull * width + col];
     acc += __shfl_xor(acc, 16, 64);
     acc += __shfl_xor(acc, 32, 64);

@@ -14,43 +14,66 @@
 // keeps at least the smallest code (2^-9 of 448), so m is never divided by eps alone because r fell under the lattice.
 #include "elem.h"
 
+#include <type_traits>
+
 namespace {
 
 constexpr int OPT_THREADS = 256;
 constexpr int OPT_BLOCK = 256;          // elements under one scale: one wave, 4 elements a lane
-constexpr int OPT_CHUNK = 4096;         // elements per workgroup: 4 passes of 256 threads x 4 elements
-constexpr int OPT_TENSORS = 36;         // tensors per launch: their descriptors travel as kernel arguments (4 KB)
-constexpr int NORM_MAX_GRID = 1024;     // partial sums per launch of the gradient norm
+// Elements per workgroup of the update: one pass of 4 a lane.  Twice and four times as many in one workgroup were slower at
+// every size (12.6 M fp32 parameters, 32 bits: 68.8 / 70.8 / 76.1 us; 8 bits: 42.2 / 43.9 / 54.1 us): more workgroups hide
+// more latency than more loads in flight in each.
+constexpr int OPT_CHUNK = OPT_THREADS * 4;
+constexpr int NORM_CHUNK = 8192;        // of the gradient norm: 8 (fp32) or 4 (16 bits) vectors a lane in flight
+constexpr uint32_t NORM_MAX_GRID = 1024;  // partial sums per launch of the gradient norm
 constexpr float E4M3_TOP = 448.f, E4M3_INV_TOP = 1.f / 448.f;
 constexpr float LEAST_TOP = 7.888609052210118e-31f;    // 2^-100: keeps 448 / top and top / 448 normal numbers
+constexpr float ROOT_MOST = 1.8446743e19f;             // sqrt of the largest float: a root stays finite in 8 bits
 constexpr float TO_LATTICE = 7.52316384526264e-37f;    // 2^-120: e4m3's exponent bias (7) in fp32's place (127)
 
-struct OptTensor {
+// Descriptors travel as kernel arguments, of which 4 KB are sure: 64 tensors with what the plain 32-bit update needs, 36 with
+// everything, 128 for the norm.  size: elements in the low 40 bits, flags above.
+struct PlainTensor {
     void *p;
     const void *g;
     void *m, *v;
-    float *sm, *sr;
-    __half *image;
-    const float *lr_dev;
-    uint64_t n, index0;
-    float lr, decay, wd;  // lr: lr / (1 - b1^t) where the step count is the host's
-    uint32_t flags;
+    uint64_t size;
+    float lr, decay;  // lr: lr / (1 - b1^t) where the step count is the host's
 };
-enum : uint32_t { DT_MASK = 3, STATE8 = 4, ALIGNED = 8 };  // flags: the type's code, and these
+struct FullTensor : PlainTensor {
+    float *sm, *sr;
+    _Float16 *image;
+    const float *lr_dev;
+    uint64_t index0;
+    float wd;
+};
+struct NormTensor { const void *g; uint64_t size; };
+constexpr int SIZE_BITS = 40;
+enum : uint32_t { DT_MASK = 3, STATE8 = 4 };  // flags: the type's code, and these
 
-struct OptLaunch {
-    OptTensor t[OPT_TENSORS];
-    uint32_t first[OPT_TENSORS];  // first chunk of each tensor
+template <class D, int MOST>
+struct Launch {
+    D t[MOST];
+    uint32_t first[MOST];  // first chunk of each tensor
     uint32_t n_tensors, n_chunks;
 };
-static_assert(sizeof(OptLaunch) <= 3840, "kernel arguments stay under 4 KB");
+using PlainLaunch = Launch<PlainTensor, 64>;
+using FullLaunch = Launch<FullTensor, 36>;
+using NormLaunch = Launch<NormTensor, 128>;
+static_assert(sizeof(PlainLaunch) <= 3840 && sizeof(FullLaunch) <= 3840 && sizeof(NormLaunch) <= 3840,
+              "kernel arguments stay under 4 KB");
 
-// the tensor that owns a chunk: one lane per tensor compares, the tensors in front of the chunk are counted
-__device__ __forceinline__ uint32_t tensor_of(const OptLaunch &a, uint32_t chunk)
+// the tensor that owns a chunk: lanes compare the tensors' first chunks, those in front of it are counted
+template <class D, int MOST>
+__device__ __forceinline__ uint32_t tensor_of(const Launch<D, MOST> &a, uint32_t chunk)
 {
-    const uint32_t lane = threadIdx.x & 63;
-    const bool before = lane < a.n_tensors && a.first[lane < a.n_tensors ? lane : 0] <= chunk;
-    return (uint32_t)__builtin_amdgcn_readfirstlane(__popcll(__ballot(before)) - 1);
+    uint32_t n = 0;
+#pragma unroll
+    for (int k = 0; k < MOST; k += 64) {
+        const uint32_t i = k + (threadIdx.x & 63);
+        n += __popcll(__ballot(i < a.n_tensors && a.first[i < MOST ? i : 0] <= chunk));
+    }
+    return (uint32_t)__builtin_amdgcn_readfirstlane(n - 1);
 }
 
 struct OptScalars { float scale, step, root, decay, b1, c1, b2, c2, eps; };  // c = 1 - b, root = 1 / sqrt(1 - b2^t)
@@ -131,136 +154,138 @@ __device__ __forceinline__ void encode_block(const float (&m)[4], const float (&
     }
 }
 
-constexpr float ROOT_MOST = 1.8446743e19f;  // sqrt of the largest float: a root stays finite in 8 bits
-
 // ---- the chunk of one workgroup ------------------------------------------------------------------------------------------
-// vector form: whole chunk inside the tensor, all pointers aligned; lane holds 4 consecutive elements
-template <int DT>
-__device__ __forceinline__ void chunk_vector(const OptTensor &t, uint64_t base, const OptScalars &s, uint32_t key0)
+template <class V, class T> __device__ __forceinline__ V get(const T *p)  // (global memory takes vectors at any element)
+{
+    V v;
+    __builtin_memcpy(&v, p, sizeof(v));
+    return v;
+}
+template <class V, class T> __device__ __forceinline__ void put(T *p, const V &v) { __builtin_memcpy(p, &v, sizeof(v)); }
+
+__device__ __forceinline__ uint32_t random_bits(uint64_t e, uint32_t key0)
+{
+    return mix32((uint32_t)e ^ (key0 + (uint32_t)(e >> 32) * 0x9e3779b9u));
+}
+
+// a whole chunk inside the tensor: a lane holds 4 consecutive elements, a wave one block of 256
+template <int DT, bool S8, class D>
+__device__ __forceinline__ void chunk_whole(const D &t, uint64_t base, const OptScalars &s, uint32_t key0)
 {
     using T = typename Elem<DT>::T;
-    using V = Vec<T, 4>;
-    V *p = reinterpret_cast<V *>((T *)t.p + base);
-    const V *g = reinterpret_cast<const V *>((const T *)t.g + base);
+    const uint64_t i = base + 4 * threadIdx.x;
+    Vec<T, 4> pv = get<Vec<T, 4>>((const T *)t.p + i);
+    const Vec<T, 4> gv = get<Vec<T, 4>>((const T *)t.g + i);
+    if constexpr (S8) {
+        const uint64_t blk = i / OPT_BLOCK;
+        const uint32_t mc = get<uint32_t>((const uint8_t *)t.m + i), rc = get<uint32_t>((const uint8_t *)t.v + i);
+        const float sm = t.sm[blk], sr = t.sr[blk];
+        float mf[4], rf[4], nm, nr;
+        uint32_t h[4], cm, cr;
+        e4m3_values(mc, mf);
+        e4m3_values(rc, rf);
 #pragma unroll
-    for (int it = 0; it < OPT_CHUNK / (OPT_THREADS * 4); ++it) {
-        const uint32_t q = it * OPT_THREADS + threadIdx.x;
-        V pv = p[q];
-        const V gv = g[q];
-        float pf[4], mf[4], vf[4], rf[4];
-        if (!(t.flags & STATE8)) {
-            float4 *mp = reinterpret_cast<float4 *>((float *)t.m + base) + q, *vp = reinterpret_cast<float4 *>((float *)t.v + base) + q;
-            *reinterpret_cast<float4 *>(mf) = *mp;
-            *reinterpret_cast<float4 *>(vf) = *vp;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                pf[k] = (float)pv.e[k];
-                adamw_elem(pf[k], mf[k], vf[k], (float)gv.e[k], s, rf[k]);
-                pv.e[k] = (T)pf[k];
-            }
-            *mp = *reinterpret_cast<float4 *>(mf);
-            *vp = *reinterpret_cast<float4 *>(vf);
-        } else {
-            const uint64_t blk = base / OPT_BLOCK + q / 64;
-            uint32_t *mp = (uint32_t *)t.m + base / 4 + q, *vp = (uint32_t *)t.v + base / 4 + q;
-            const uint32_t mc = *mp, rc = *vp;
-            const float sm = t.sm[blk], sr = t.sr[blk];
-            const uint64_t e = t.index0 + base + 4 * (uint64_t)q;
-            const uint32_t key = key0 + (uint32_t)(e >> 32) * 0x9e3779b9u;
-            uint32_t h[4];
-            e4m3_values(mc, mf);
-            e4m3_values(rc, rf);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                pf[k] = (float)pv.e[k];
-                mf[k] *= sm;
-                rf[k] *= sr;
-                vf[k] = rf[k] * rf[k];
-                adamw_elem(pf[k], mf[k], vf[k], (float)gv.e[k], s, rf[k]);
-                rf[k] = fminf(rf[k], ROOT_MOST);
-                pv.e[k] = (T)pf[k];
-                h[k] = mix32(((uint32_t)e + k) ^ key);
-            }
-            uint32_t cm, cr;
-            float nm, nr;
-            encode_block(mf, rf, h, cm, cr, nm, nr);
-            *mp = cm;
-            *vp = cr;
-            if ((threadIdx.x & 63) == 0) { t.sm[blk] = nm; t.sr[blk] = nr; }
+        for (int k = 0; k < 4; ++k) {
+            float pf = (float)pv.e[k], vf = rf[k] * sr;
+            mf[k] *= sm;
+            vf *= vf;
+            adamw_elem(pf, mf[k], vf, (float)gv.e[k], s, rf[k]);
+            rf[k] = fminf(rf[k], ROOT_MOST);
+            pv.e[k] = (T)pf;
+            h[k] = random_bits(t.index0 + i + k, key0);
         }
-        p[q] = pv;
+        encode_block(mf, rf, h, cm, cr, nm, nr);
+        put((uint8_t *)t.m + i, cm);
+        put((uint8_t *)t.v + i, cr);
+        if ((threadIdx.x & 63) == 0) { t.sm[blk] = nm; t.sr[blk] = nr; }
+    } else {
+        Vec<float, 4> m = get<Vec<float, 4>>((const float *)t.m + i), v = get<Vec<float, 4>>((const float *)t.v + i);
+        float r;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            float pf = (float)pv.e[k];
+            adamw_elem(pf, m.e[k], v.e[k], (float)gv.e[k], s, r);
+            pv.e[k] = (T)pf;
+        }
+        put((float *)t.m + i, m);
+        put((float *)t.v + i, v);
+    }
+    put((T *)t.p + i, pv);
+    if constexpr (std::is_same<D, FullTensor>::value)
         if (t.image) {
             Vec<_Float16, 4> hv;
 #pragma unroll
             for (int k = 0; k < 4; ++k) hv.e[k] = (_Float16)(float)pv.e[k];
-            reinterpret_cast<Vec<_Float16, 4> *>((_Float16 *)t.image + base)[q] = hv;
+            put(t.image + i, hv);
         }
-    }
 }
 
-// element form: the tensor's last chunk, or pointers that no vector load takes; lanes hold elements 64 apart
-template <int DT>
-__device__ __forceinline__ void chunk_element(const OptTensor &t, uint64_t base, const OptScalars &s, uint32_t key0)
+// the tensor's last chunk: a wave has its block of 256 all the same, its lanes hold elements 64 apart
+template <int DT, bool S8, class D>
+__device__ __forceinline__ void chunk_last(const D &t, uint64_t base, uint64_t n, const OptScalars &s, uint32_t key0)
 {
     using T = typename Elem<DT>::T;
-    T *p = (T *)t.p;
-    const T *g = (const T *)t.g;
-    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    for (int it = 0; it < OPT_CHUNK / (OPT_THREADS * 4); ++it) {
-        const uint64_t b0 = base + (it * 4 + wave) * (uint64_t)OPT_BLOCK;
-        if (b0 >= t.n) return;  // (the whole wave leaves)
-        float mf[4], rf[4];
-        uint32_t h[4];
-        const uint64_t blk = b0 / OPT_BLOCK;
-        const float sm = t.flags & STATE8 ? t.sm[blk] : 0.f, sr = t.flags & STATE8 ? t.sr[blk] : 0.f;
+    const uint32_t lane = threadIdx.x & 63;
+    const uint64_t b0 = base + (threadIdx.x >> 6) * OPT_BLOCK, blk = b0 / OPT_BLOCK;
+    if (b0 >= n) return;  // (the whole wave)
+    float mf[4], rf[4], sm = 0.f, sr = 0.f;
+    uint32_t h[4];
+    if constexpr (S8) { sm = t.sm[blk]; sr = t.sr[blk]; }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const uint64_t i = b0 + k * 64 + lane;
+        mf[k] = rf[k] = 0.f;
+        h[k] = 0;
+        if (i >= n) continue;
+        float pf = (float)((const T *)t.p)[i], vf;
+        if constexpr (S8) {
+            mf[k] = e4m3_value(((const uint8_t *)t.m)[i]) * sm;
+            vf = e4m3_value(((const uint8_t *)t.v)[i]) * sr;
+            vf *= vf;
+            h[k] = random_bits(t.index0 + i, key0);
+        } else {
+            mf[k] = ((const float *)t.m)[i];
+            vf = ((const float *)t.v)[i];
+        }
+        adamw_elem(pf, mf[k], vf, (float)((const T *)t.g)[i], s, rf[k]);
+        rf[k] = fminf(rf[k], ROOT_MOST);
+        const T pt = (T)pf;
+        ((T *)t.p)[i] = pt;
+        if constexpr (std::is_same<D, FullTensor>::value)
+            if (t.image) t.image[i] = (_Float16)(float)pt;
+        if constexpr (!S8) {
+            ((float *)t.m)[i] = mf[k];
+            ((float *)t.v)[i] = vf;
+        }
+    }
+    if constexpr (S8) {
+        uint32_t cm, cr;
+        float nm, nr;
+        encode_block(mf, rf, h, cm, cr, nm, nr);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const uint64_t i = b0 + k * 64 + lane;
-            mf[k] = rf[k] = 0.f;
-            h[k] = 0;
-            if (i >= t.n) continue;
-            float pf = (float)p[i], vf;
-            if (t.flags & STATE8) {
-                mf[k] = e4m3_value(((const uint8_t *)t.m)[i]) * sm;
-                const float r0 = e4m3_value(((const uint8_t *)t.v)[i]) * sr;
-                vf = r0 * r0;
-                const uint64_t e = t.index0 + i;
-                h[k] = mix32((uint32_t)e ^ (key0 + (uint32_t)(e >> 32) * 0x9e3779b9u));
-            } else {
-                mf[k] = ((const float *)t.m)[i];
-                vf = ((const float *)t.v)[i];
-            }
-            adamw_elem(pf, mf[k], vf, (float)g[i], s, rf[k]);
-            rf[k] = fminf(rf[k], ROOT_MOST);
-            const T pt = (T)pf;
-            p[i] = pt;
-            if (t.image) ((_Float16 *)t.image)[i] = (_Float16)(float)pt;
-            if (!(t.flags & STATE8)) {
-                ((float *)t.m)[i] = mf[k];
-                ((float *)t.v)[i] = vf;
+            if (i < n) {
+                ((uint8_t *)t.m)[i] = (uint8_t)(cm >> (8 * k));
+                ((uint8_t *)t.v)[i] = (uint8_t)(cr >> (8 * k));
             }
         }
-        if (t.flags & STATE8) {
-            uint32_t cm, cr;
-            float nm, nr;
-            encode_block(mf, rf, h, cm, cr, nm, nr);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const uint64_t i = b0 + k * 64 + lane;
-                if (i < t.n) {
-                    ((uint8_t *)t.m)[i] = (uint8_t)(cm >> (8 * k));
-                    ((uint8_t *)t.v)[i] = (uint8_t)(cr >> (8 * k));
-                }
-            }
-            if (lane == 0) { t.sm[blk] = nm; t.sr[blk] = nr; }
-        }
+        if (lane == 0) { t.sm[blk] = nm; t.sr[blk] = nr; }
     }
 }
 
-// hyper of nsr_adamw_begin: {gradient factor, 1 / (1 - b1^t), 1 / sqrt(1 - b2^t), leave out?, t, norm}
-__global__ void __launch_bounds__(OPT_THREADS)
-k_adamw_tensors(const OptLaunch a, OptScalars s, uint32_t seed, uint32_t step, const float *__restrict__ hyper)
+template <int DT, bool S8, class D>
+__device__ __forceinline__ void run_chunk(const D &t, uint64_t base, uint64_t n, const OptScalars &s, uint32_t key0)
 {
+    base + OPT_CHUNK <= n ? chunk_whole<DT, S8>(t, base, s, key0) : chunk_last<DT, S8>(t, base, n, s, key0);
+}
+
+// hyper of nsr_adamw_begin: {gradient factor, 1 / (1 - b1^t), 1 / sqrt(1 - b2^t), leave out?, t, norm}
+template <class D, int MOST>
+__global__ void __launch_bounds__(OPT_THREADS)
+k_adamw_tensors(const Launch<D, MOST> a, OptScalars s, uint32_t seed, uint32_t step, const float *__restrict__ hyper)
+{
+    constexpr bool FULL = std::is_same<D, FullTensor>::value;
     if (hyper) {
         if (__float_as_int(hyper[3])) return;
         s.scale *= hyper[0];
@@ -268,80 +293,100 @@ k_adamw_tensors(const OptLaunch a, OptScalars s, uint32_t seed, uint32_t step, c
         step = (uint32_t)__float_as_int(hyper[4]);
     }
     const uint32_t which = tensor_of(a, blockIdx.x);
-    const OptTensor &t = a.t[which];
+    const D &t = a.t[which];
+    const uint32_t flags = (uint32_t)(t.size >> SIZE_BITS);
+    const uint64_t n = t.size & ((1ull << SIZE_BITS) - 1), base = (uint64_t)(blockIdx.x - a.first[which]) * OPT_CHUNK;
     float lr = t.lr;
     s.decay = t.decay;
-    if (t.lr_dev) {
-        lr = *t.lr_dev;
-        s.decay = 1.f - lr * t.wd;
+    uint32_t key0 = 0;
+    if constexpr (FULL) {
+        if (t.lr_dev) {
+            lr = *t.lr_dev;
+            s.decay = 1.f - lr * t.wd;
+        }
+        key0 = mix32(mix32(step) ^ seed);
     }
     s.step = hyper ? lr * hyper[1] : lr;
-    const uint32_t key0 = mix32(mix32(step) ^ seed);
-    const uint64_t base = (uint64_t)(blockIdx.x - a.first[which]) * OPT_CHUNK;
-    const bool vec = (t.flags & ALIGNED) && base + OPT_CHUNK <= t.n;
-    switch (t.flags & DT_MASK) {
-    case DT_F32: vec ? chunk_vector<DT_F32>(t, base, s, key0) : chunk_element<DT_F32>(t, base, s, key0); break;
-    case DT_F16: vec ? chunk_vector<DT_F16>(t, base, s, key0) : chunk_element<DT_F16>(t, base, s, key0); break;
-    default: vec ? chunk_vector<DT_BF16>(t, base, s, key0) : chunk_element<DT_BF16>(t, base, s, key0); break;
-    }
+    const uint32_t dt = flags & DT_MASK;
+    if constexpr (FULL)
+        if (flags & STATE8) {
+            if (dt == DT_F32) run_chunk<DT_F32, true>(t, base, n, s, key0);
+            else if (dt == DT_F16) run_chunk<DT_F16, true>(t, base, n, s, key0);
+            else run_chunk<DT_BF16, true>(t, base, n, s, key0);
+            return;
+        }
+    if (dt == DT_F32) run_chunk<DT_F32, false>(t, base, n, s, key0);
+    else if (dt == DT_F16) run_chunk<DT_F16, false>(t, base, n, s, key0);
+    else run_chunk<DT_BF16, false>(t, base, n, s, key0);
 }
 
 // ---- norm of all gradients -----------------------------------------------------------------------------------------------
 // squares and sums in 64 bits: no overflow for any finite gradient, and the same value for every order that matters in fp32
 template <int DT>
-__device__ __forceinline__ double chunk_squares(const OptTensor &t, uint64_t base)
+__device__ __forceinline__ double chunk_squares(const void *grad, uint64_t n, uint64_t base)
 {
     using T = typename Elem<DT>::T;
-    const T *g = (const T *)t.g + base;
-    const uint64_t left = t.n - base;
-    double acc = 0.0;
-    if ((t.flags & ALIGNED) && left >= OPT_CHUNK) {
-        Vec<T, 4> v[4];
+    constexpr int N = 16 / sizeof(T), PASSES = NORM_CHUNK / (OPT_THREADS * N);
+    const T *g = (const T *)grad + base;
+    double acc[2] = {0.0, 0.0};  // (two chains of additions)
+    if (n - base >= NORM_CHUNK) {
+        Vec<T, N> v[PASSES];
 #pragma unroll
-        for (int it = 0; it < 4; ++it) v[it] = reinterpret_cast<const Vec<T, 4> *>(g)[it * OPT_THREADS + threadIdx.x];
+        for (int it = 0; it < PASSES; ++it) v[it] = get<Vec<T, N>>(g + (it * OPT_THREADS + threadIdx.x) * N);
 #pragma unroll
-        for (int it = 0; it < 4; ++it)
+        for (int it = 0; it < PASSES; ++it)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) { const double d = (double)v[it].e[k]; acc += d * d; }
+            for (int k = 0; k < N; ++k) { const double d = (double)(float)v[it].e[k]; acc[k & 1] = fma(d, d, acc[k & 1]); }
     } else {
-        const uint32_t n = left < OPT_CHUNK ? (uint32_t)left : OPT_CHUNK;
-        for (uint32_t i = threadIdx.x; i < n; i += OPT_THREADS) { const double d = (double)g[i]; acc += d * d; }
+        for (uint32_t i = threadIdx.x; i < (uint32_t)(n - base); i += OPT_THREADS) {
+            const double d = (double)(float)g[i];
+            acc[0] = fma(d, d, acc[0]);
+        }
     }
-    return acc;
+    return acc[0] + acc[1];
+}
+
+__device__ __forceinline__ double wave_sum64(double v)
+{
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
 }
 
 __global__ void __launch_bounds__(OPT_THREADS)
-k_grad_squares(const OptLaunch a, double *__restrict__ partials)
+k_grad_squares(const NormLaunch a, double *__restrict__ partials)
 {
     double acc = 0.0;
     for (uint32_t chunk = blockIdx.x; chunk < a.n_chunks; chunk += gridDim.x) {
         const uint32_t which = tensor_of(a, chunk);
-        const OptTensor &t = a.t[which];
-        const uint64_t base = (uint64_t)(chunk - a.first[which]) * OPT_CHUNK;
-        switch (t.flags & DT_MASK) {
-        case DT_F32: acc += chunk_squares<DT_F32>(t, base); break;
-        case DT_F16: acc += chunk_squares<DT_F16>(t, base); break;
-        default: acc += chunk_squares<DT_BF16>(t, base); break;
-        }
+        const NormTensor &t = a.t[which];
+        const uint64_t n = t.size & ((1ull << SIZE_BITS) - 1), base = (uint64_t)(chunk - a.first[which]) * NORM_CHUNK;
+        const uint32_t dt = (uint32_t)(t.size >> SIZE_BITS) & DT_MASK;
+        if (dt == DT_F32) acc += chunk_squares<DT_F32>(t.g, n, base);
+        else if (dt == DT_F16) acc += chunk_squares<DT_F16>(t.g, n, base);
+        else acc += chunk_squares<DT_BF16>(t.g, n, base);
     }
     __shared__ double part[OPT_THREADS / 64];
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) acc += __shfl_xor(acc, o, 64);
+    acc = wave_sum64(acc);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = acc;
     __syncthreads();
     if (threadIdx.x == 0) partials[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-// one workgroup: the partial sums in a fixed order, then the step's scalars
-__global__ void __launch_bounds__(OPT_THREADS)
-k_adamw_begin(int32_t *__restrict__ step, float *__restrict__ hyper, double b1, double b2, const double *__restrict__ partials,
-              uint32_t n_partials, double max_norm, const float *__restrict__ grad_scale, const float *__restrict__ found_inf)
+// one workgroup: the partial sums in a fixed order, then the step's scalars.  Two threads have worked out b^t = exp(t ln b) in 64
+// bits meanwhile (its error, t |ln b| 2^-53 of it, is far under fp32's; pow took twice as long as the whole kernel does now).
+constexpr int BEGIN_THREADS = 1024;
+__global__ void __launch_bounds__(BEGIN_THREADS)
+k_adamw_begin(int32_t *__restrict__ step, float *__restrict__ hyper, double ln_b1, double ln_b2,
+              const double *__restrict__ partials, uint32_t n_partials, double max_norm, const float *__restrict__ grad_scale,
+              const float *__restrict__ found_inf)
 {
+    __shared__ double part[BEGIN_THREADS / 64], power[2];
+    const int32_t taken = *step;
     double acc = 0.0;
-    for (uint32_t i = threadIdx.x; i < n_partials; i += OPT_THREADS) acc += partials[i];
-    __shared__ double part[OPT_THREADS / 64];
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) acc += __shfl_xor(acc, o, 64);
+    for (uint32_t i = threadIdx.x; i < n_partials; i += BEGIN_THREADS) acc += partials[i];
+    if (threadIdx.x == 64 || threadIdx.x == 128) power[threadIdx.x / 128] = exp((taken + 1.0) * (threadIdx.x == 64 ? ln_b1 : ln_b2));
+    acc = wave_sum64(acc);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = acc;
     __syncthreads();
     if (threadIdx.x != 0) return;
@@ -349,41 +394,45 @@ k_adamw_begin(int32_t *__restrict__ step, float *__restrict__ hyper, double b1, 
     double factor = unscale;
     bool skip = found_inf && *found_inf != 0.f;
     if (partials) {
-        const double norm = sqrt((part[0] + part[1]) + (part[2] + part[3])) * unscale;
+        double sum = part[0];
+        for (int k = 1; k < BEGIN_THREADS / 64; ++k) sum += part[k];
+        const double norm = sqrt(sum) * unscale;
         const double ratio = max_norm / (norm + 1e-6);  // torch.nn.utils.clip_grad_norm_
         factor *= ratio < 1.0 ? ratio : 1.0;
         skip = skip || !(norm <= 1.7976931348623157e308);
         hyper[5] = (float)norm;
     }
-    const int32_t t = skip ? *step : *step + 1;
-    if (!skip) *step = t;
+    if (!skip) *step = taken + 1;
     hyper[0] = (float)factor;
-    hyper[1] = (float)(1.0 / (1.0 - pow(b1, (double)t)));
-    hyper[2] = (float)(1.0 / sqrt(1.0 - pow(b2, (double)t)));
+    hyper[1] = (float)(1.0 / (1.0 - power[0]));
+    hyper[2] = (float)(1.0 / sqrt(1.0 - power[1]));
     hyper[3] = __int_as_float(skip ? 1 : 0);
-    hyper[4] = __int_as_float(t);
+    hyper[4] = __int_as_float(taken + 1);  // (read only where the step is taken)
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------------
-bool all_aligned(const OptTensor &t)
-{
-    const uintptr_t own = (uintptr_t)t.p | (uintptr_t)t.g, state = (uintptr_t)t.m | (uintptr_t)t.v;
-    const uintptr_t need = (t.flags & DT_MASK) == DT_F32 ? 15 : 7, need_state = t.flags & STATE8 ? 3 : 15;
-    return (own & need) == 0 && (state & need_state) == 0 && ((uintptr_t)t.image & 7) == 0;
-}
+// 2^23 chunks of 256 threads are 2^31 threads: a grid stays under the launch limit of 2^32 with the next tensor's chunks too.
+// A tensor of more chunks is several pieces.
+constexpr uint32_t LAUNCH_CHUNKS = 1u << 23;
 
-// fills launches of at most OPT_TENSORS tensors and hands each to `go`; grads_only: the norm, which reads nothing else
-template <class Go>
-int each_launch(const char *what, const NsrAdamwTensor *tensors, uint32_t n_tensors, bool grads_only, bool lr_on_device, double b1_correction, Go go)
+int check_grads(const char *what, const NsrAdamwTensor *tensors, uint32_t n_tensors)
 {
     NSR_REQUIRE(n_tensors == 0 || tensors, "%s: NULL descriptors", what);
-    for (uint32_t i = 0; i < n_tensors; ++i) {  // refuse before anything is launched
+    for (uint32_t i = 0; i < n_tensors; ++i) {
         const NsrAdamwTensor &x = tensors[i];
         NSR_REQUIRE(x.n < (1ull << 35), "%s: tensor %u has 2^35 elements or more", what, i);
-        NSR_REQUIRE(x.dtype <= 2, "%s: tensor %u: dtype %u (0 fp32, 1 fp16, 2 bf16)", what, i, x.dtype);
+        NSR_REQUIRE(x.dtype <= DT_BF16, "%s: tensor %u: dtype %u (0 fp32, 1 fp16, 2 bf16)", what, i, x.dtype);
         NSR_REQUIRE(x.n == 0 || x.grad, "%s: tensor %u has a NULL gradient", what, i);
-        NSR_REQUIRE(((uintptr_t)x.grad & (x.dtype == 0 ? 3 : 1)) == 0, "%s: tensor %u: misaligned gradient", what, i);
-        if (grads_only || x.n == 0) continue;
+        NSR_REQUIRE(((uintptr_t)x.grad & (dtype_size(x.dtype) - 1)) == 0, "%s: tensor %u: misaligned gradient", what, i);
+    }
+    return NSR_OK;
+}
+
+int check_states(const char *what, const NsrAdamwTensor *tensors, uint32_t n_tensors, bool lr_on_device)
+{
+    for (uint32_t i = 0; i < n_tensors; ++i) {
+        const NsrAdamwTensor &x = tensors[i];
+        if (x.n == 0) continue;
         NSR_REQUIRE(x.params && x.exp_avg && x.exp_avg_sq, "%s: tensor %u has a NULL pointer", what, i);
         NSR_REQUIRE(x.state_bits == 32 || x.state_bits == 8, "%s: tensor %u: moments in %u bits (32 or 8)", what, i, x.state_bits);
         NSR_REQUIRE(x.state_bits == 32 || (x.scales_m && x.scales_r), "%s: tensor %u: 8-bit moments need scales", what, i);
@@ -391,33 +440,34 @@ int each_launch(const char *what, const NsrAdamwTensor *tensors, uint32_t n_tens
         NSR_REQUIRE(x.index0 % OPT_BLOCK == 0, "%s: tensor %u: index0 must be a multiple of %d", what, i, OPT_BLOCK);
         const uintptr_t fp32 = (uintptr_t)x.scales_m | (uintptr_t)x.scales_r | (uintptr_t)x.lr_dev |
                                (x.state_bits == 32 ? (uintptr_t)x.exp_avg | (uintptr_t)x.exp_avg_sq : 0);
-        NSR_REQUIRE((fp32 & 3) == 0 && ((uintptr_t)x.params & (x.dtype == 0 ? 3 : 1)) == 0 && ((uintptr_t)x.image & 1) == 0,
+        NSR_REQUIRE((fp32 & 3) == 0 && ((uintptr_t)x.params & (dtype_size(x.dtype) - 1)) == 0 && ((uintptr_t)x.image & 1) == 0,
                     "%s: tensor %u: misaligned pointer", what, i);
     }
-    OptLaunch a;
+    return NSR_OK;
+}
+
+// fills launches of at most MOST tensors (or pieces of tensors: fill(descriptor, tensor, first element, elements)) and hands
+// each to `go`
+template <class D, int MOST, class Fill, class Go>
+int each_launch(const NsrAdamwTensor *tensors, uint32_t n_tensors, uint32_t chunk, Fill fill, Go go)
+{
+    Launch<D, MOST> a;
     a.n_tensors = a.n_chunks = 0;
     for (uint32_t i = 0; i < n_tensors; ++i) {
-        const NsrAdamwTensor &x = tensors[i];
-        if (x.n) {
-            OptTensor &t = a.t[a.n_tensors];
-            t.p = x.params; t.g = x.grad; t.m = x.exp_avg; t.v = x.exp_avg_sq;
-            t.sm = x.scales_m; t.sr = x.scales_r; t.image = (__half *)x.image; t.lr_dev = x.lr_dev;
-            t.n = x.n; t.index0 = x.index0;
-            t.lr = (float)(x.lr / b1_correction); t.decay = (float)(1.0 - x.lr * x.weight_decay); t.wd = (float)x.weight_decay;
-            t.flags = x.dtype | (x.state_bits == 8 ? STATE8 : 0);
-            if (grads_only) t.flags |= ((uintptr_t)x.grad & (x.dtype == 0 ? 15 : 7)) == 0 ? ALIGNED : 0;
-            else t.flags |= all_aligned(t) ? ALIGNED : 0;
+        const uint64_t n = tensors[i].n, most = (uint64_t)LAUNCH_CHUNKS * chunk;
+        for (uint64_t at = 0; at < n; at += most) {
+            const uint64_t part = n - at < most ? n - at : most;
+            fill(a.t[a.n_tensors], tensors[i], at, part);
             a.first[a.n_tensors++] = a.n_chunks;
-            a.n_chunks += nsr_div_up(x.n, OPT_CHUNK);
-        }
-        // 2^23 chunks are 2^31 threads: the grid stays under the launch limit (2^32 threads) with the next tensor's 2^23 more
-        if (a.n_tensors && (a.n_tensors == OPT_TENSORS || a.n_chunks >= (1u << 23) - 1 || i + 1 == n_tensors)) {
-            const int rc = go(a);
-            if (rc != NSR_OK) return rc;
-            a.n_tensors = a.n_chunks = 0;
+            a.n_chunks += nsr_div_up(part, chunk);
+            if (a.n_tensors == MOST || a.n_chunks >= LAUNCH_CHUNKS - 1) {
+                const int rc = go(a);
+                if (rc != NSR_OK) return rc;
+                a.n_tensors = a.n_chunks = 0;
+            }
         }
     }
-    return NSR_OK;
+    return a.n_tensors ? go(a) : NSR_OK;
 }
 
 }  // namespace
@@ -428,26 +478,46 @@ extern "C" int nsr_adamw_tensors(const NsrAdamwTensor *tensors, uint32_t n_tenso
     NSR_REQUIRE(hyper || step >= 1, "nsr_adamw_tensors: step counts from 1");
     NSR_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "nsr_adamw_tensors: betas in [0, 1)");
     NSR_REQUIRE(eps >= 0.0, "nsr_adamw_tensors: eps >= 0");
-    double c1 = 1.0, c2 = 1.0;
-    if (!hyper) { c1 = 1.0 - pow(beta1, (double)step); c2 = 1.0 - pow(beta2, (double)step); }
+    int rc = check_grads("nsr_adamw_tensors", tensors, n_tensors);
+    if (rc == NSR_OK) rc = check_states("nsr_adamw_tensors", tensors, n_tensors, hyper != nullptr);
+    if (rc != NSR_OK) return rc;
+    const double c1 = hyper ? 1.0 : 1.0 - pow(beta1, (double)step), c2 = hyper ? 1.0 : 1.0 - pow(beta2, (double)step);
     OptScalars s;
     s.scale = (float)grad_unscale; s.step = 0.f; s.root = (float)(1.0 / sqrt(c2)); s.decay = 1.f;
     s.b1 = (float)beta1; s.c1 = (float)(1.0 - beta1); s.b2 = (float)beta2; s.c2 = (float)(1.0 - beta2); s.eps = (float)eps;
-    return each_launch("nsr_adamw_tensors", tensors, n_tensors, false, hyper != nullptr, c1, [&](const OptLaunch &a) {
-        hipLaunchKernelGGL(k_adamw_tensors, dim3(a.n_chunks), dim3(OPT_THREADS), 0, (hipStream_t)stream, a, s, seed,
-                           (uint32_t)step, hyper);
+    bool plain = true;
+    for (uint32_t i = 0; i < n_tensors; ++i)
+        plain = plain && (tensors[i].n == 0 || (tensors[i].state_bits == 32 && !tensors[i].image && !tensors[i].lr_dev));
+    auto fill = [&](PlainTensor &t, const NsrAdamwTensor &x, uint64_t at, uint64_t n) {
+        const uint64_t e = at * dtype_size(x.dtype), st = at * x.state_bits / 8;
+        t.p = (char *)x.params + e; t.g = (const char *)x.grad + e; t.m = (char *)x.exp_avg + st; t.v = (char *)x.exp_avg_sq + st;
+        t.size = n | (uint64_t)(x.dtype | (x.state_bits == 8 ? STATE8 : 0)) << SIZE_BITS;
+        t.lr = (float)(x.lr / c1); t.decay = (float)(1.0 - x.lr * x.weight_decay);
+    };
+    auto fill_all = [&](FullTensor &t, const NsrAdamwTensor &x, uint64_t at, uint64_t n) {
+        fill(t, x, at, n);
+        t.sm = x.scales_m ? x.scales_m + at / OPT_BLOCK : nullptr; t.sr = x.scales_r ? x.scales_r + at / OPT_BLOCK : nullptr;
+        t.image = x.image ? (_Float16 *)x.image + at : nullptr; t.lr_dev = x.lr_dev;
+        t.index0 = x.index0 + at; t.wd = (float)x.weight_decay;
+    };
+    auto go = [&](const auto &a, auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(a.n_chunks), dim3(OPT_THREADS), 0, (hipStream_t)stream, a, s, seed, (uint32_t)step, hyper);
         NSR_CHECK_LAUNCH("nsr_adamw_tensors");
         return NSR_OK;
-    });
+    };
+    if (plain)
+        return each_launch<PlainTensor, 64>(tensors, n_tensors, OPT_CHUNK, fill,
+                                            [&](const PlainLaunch &a) { return go(a, k_adamw_tensors<PlainTensor, 64>); });
+    return each_launch<FullTensor, 36>(tensors, n_tensors, OPT_CHUNK, fill_all,
+                                       [&](const FullLaunch &a) { return go(a, k_adamw_tensors<FullTensor, 36>); });
 }
 
 extern "C" uint32_t nsr_grad_squares_capacity(const NsrAdamwTensor *tensors, uint32_t n_tensors)
 {
-    // a launch ends after OPT_TENSORS tensors or 2^23 - 1 chunks, whichever comes first
+    // a launch ends after 128 tensors (or pieces) or LAUNCH_CHUNKS - 1 chunks, whichever comes first
     uint64_t chunks = 0;
-    for (uint32_t i = 0; tensors && i < n_tensors; ++i) chunks += nsr_div_up(tensors[i].n, OPT_CHUNK);
-    const uint64_t launches = nsr_div_up(n_tensors, OPT_TENSORS) + chunks / ((1u << 23) - 1) + 1;
-    return (uint32_t)(launches * NORM_MAX_GRID);
+    for (uint32_t i = 0; tensors && i < n_tensors; ++i) chunks += nsr_div_up(tensors[i].n, NORM_CHUNK);
+    return (uint32_t)((nsr_div_up(n_tensors, 128) + 2 * (chunks / (LAUNCH_CHUNKS - 1)) + 1) * NORM_MAX_GRID);
 }
 
 extern "C" int nsr_grad_squares(const NsrAdamwTensor *tensors, uint32_t n_tensors, double *partials, uint32_t capacity,
@@ -456,8 +526,14 @@ extern "C" int nsr_grad_squares(const NsrAdamwTensor *tensors, uint32_t n_tensor
     NSR_REQUIRE(partials && n_partials, "nsr_grad_squares: NULL pointer");
     NSR_REQUIRE(((uintptr_t)partials & 7) == 0, "nsr_grad_squares: partials must be 8-byte aligned");
     *n_partials = 0;
-    return each_launch("nsr_grad_squares", tensors, n_tensors, true, true, 1.0, [&](const OptLaunch &a) {
-        const uint32_t grid = a.n_chunks < (uint32_t)NORM_MAX_GRID ? a.n_chunks : NORM_MAX_GRID;
+    const int rc = check_grads("nsr_grad_squares", tensors, n_tensors);
+    if (rc != NSR_OK) return rc;
+    auto fill = [](NormTensor &t, const NsrAdamwTensor &x, uint64_t at, uint64_t n) {
+        t.g = (const char *)x.grad + at * dtype_size(x.dtype);
+        t.size = n | (uint64_t)x.dtype << SIZE_BITS;
+    };
+    return each_launch<NormTensor, 128>(tensors, n_tensors, NORM_CHUNK, fill, [&](const NormLaunch &a) {
+        const uint32_t grid = a.n_chunks < NORM_MAX_GRID ? a.n_chunks : NORM_MAX_GRID;
         NSR_REQUIRE(capacity - *n_partials >= grid, "nsr_grad_squares: room for %u partial sums is too little", capacity);
         hipLaunchKernelGGL(k_grad_squares, dim3(grid), dim3(OPT_THREADS), 0, (hipStream_t)stream, a, partials + *n_partials);
         NSR_CHECK_LAUNCH("nsr_grad_squares");
@@ -473,8 +549,8 @@ extern "C" int nsr_adamw_begin(int32_t *step, float *hyper, double beta1, double
     NSR_REQUIRE(step && hyper, "nsr_adamw_begin: NULL pointer");
     NSR_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "nsr_adamw_begin: betas in [0, 1)");
     NSR_REQUIRE(!partials || max_norm > 0.0, "nsr_adamw_begin: max_norm > 0");
-    hipLaunchKernelGGL(k_adamw_begin, dim3(1), dim3(OPT_THREADS), 0, (hipStream_t)stream, step, hyper, beta1, beta2, partials,
-                       partials ? n_partials : 0, max_norm, grad_scale, found_inf);
+    hipLaunchKernelGGL(k_adamw_begin, dim3(1), dim3(BEGIN_THREADS), 0, (hipStream_t)stream, step, hyper, log(beta1), log(beta2),
+                       partials, partials ? n_partials : 0, max_norm, grad_scale, found_inf);
     NSR_CHECK_LAUNCH("nsr_adamw_begin");
     return NSR_OK;
 }

@@ -92,7 +92,8 @@ class AdamW(torch.optim.Optimizer):
         self.device = items[0][0].device
         self._ps = [p for p, _ in items]
         self._group_of = [i for _, i in items]
-        self._dense = [p.is_contiguous() for p in self._ps]
+        self._all_contiguous = all(p.is_contiguous() for p in self._ps)
+        self._addresses = [p.data_ptr() for p in self._ps]
         self._bits = [8 if self.state_bits == 8 and p.numel() >= self.min_8bit_size else 32 for p in self._ps]
         self._at, total = [], {8: 0, 32: 0}
         for p, bits in zip(self._ps, self._bits):
@@ -110,7 +111,7 @@ class AdamW(torch.optim.Optimizer):
         self._fields = np.frombuffer(self._desc, dtype=np.dtype(NsrAdamwTensor))
         f = self._fields
         f["n"] = [p.numel() for p in self._ps]
-        f["params"] = [p.data_ptr() for p in self._ps]
+        f["params"] = self._addresses
         f["dtype"] = [DTYPE_CODES[p.dtype] for p in self._ps]
         f["state_bits"] = self._bits
         f["index0"] = self._at
@@ -212,34 +213,33 @@ class AdamW(torch.optim.Optimizer):
     # ---- one step ------------------------------------------------------------------------------------------------------------
     def _gather(self):
         """this step's addresses in the descriptors; (host array, count, live parameters, tensors to keep until the launch)"""
-        f, live, keep = self._fields, [], []
-        grads, params = [], []
-        for i, p in enumerate(self._ps):
-            g = p.grad
-            if g is None:
-                continue
-            if not g.is_contiguous() or not self._dense[i]:
+        f, ps = self._fields, self._ps
+        grads = [p.grad for p in ps]
+        addresses = [p.data_ptr() for p in ps]
+        if addresses != self._addresses:
+            self._check_moved()
+            self._addresses = addresses
+            f["params"] = addresses
+        keep = []
+        if not self._all_contiguous or any([g is None or not g.is_contiguous() for g in grads]):
+            for i, (p, g) in enumerate(zip(ps, grads)):
+                if g is None:
+                    continue
                 if g.is_sparse:
                     raise NsrError("AdamW: sparse gradients are not supported")
-                if g.stride() != p.stride():
-                    keep.append(torch.empty_strided(p.shape, p.stride(), dtype=p.dtype, device=p.device).copy_(g))
-                    g = keep[-1]
-            live.append(i)
-            grads.append(g.data_ptr())
-            params.append(p.data_ptr())
-        if len(live) == len(self._ps):
-            f["grad"], old = grads, f["params"].copy()
-            f["params"] = params
-            if not np.array_equal(f["params"], old):
-                self._check_moved()
-            return self._desc, len(live), self._ps, keep
-        for i, g, a in zip(live, grads, params):
-            f["grad"][i] = g
-            if f["params"][i] != a:
-                f["params"][i] = a
-                self._check_moved()
-        some = f[live]  # (a copy)
-        return some.ctypes.data, len(live), [self._ps[i] for i in live], keep + [some]
+                if g.stride() != p.stride() and p.numel():  # in the parameter's order of elements
+                    grads[i] = torch.empty_strided(p.shape, p.stride(), dtype=p.dtype, device=p.device)
+                    with torch.no_grad():
+                        grads[i].copy_(g)
+            keep = grads
+            live = [i for i, g in enumerate(grads) if g is not None]
+            if len(live) < len(ps):
+                for i in live:
+                    f["grad"][i] = grads[i].data_ptr()
+                some = f[live]  # (a copy)
+                return some.ctypes.data, len(live), [ps[i] for i in live], (keep, some)
+        f["grad"] = [g.data_ptr() for g in grads]
+        return self._desc, len(ps), ps, keep
 
     def _check_moved(self):
         """parameters whose memory was replaced (``p.data = ...``) still have the layout that the moments were made for"""
@@ -251,7 +251,6 @@ class AdamW(torch.optim.Optimizer):
     def _stride(self, i):
         return next(iter(self.state[self._ps[i]].values())).stride()
 
-    @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:
@@ -279,7 +278,7 @@ class AdamW(torch.optim.Optimizer):
             for m, i, image in self._images:
                 p = m.params
                 if m._shadow is not image or not m._shadow_trusted or m._shadow_key != (p.data_ptr(), p._version, p.device):
-                    image.copy_(p)  # first step, or the parameters were written from outside
+                    image.copy_(p.detach())  # first step, or the parameters were written from outside
             s = stream_ptr()
             if self._step_dev is None:
                 self._step += 1

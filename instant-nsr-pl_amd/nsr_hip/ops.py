@@ -866,20 +866,26 @@ def _ln_check(x, weight, bias):
     return x.dtype if affine is None else affine
 
 
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
 def _layer_norm(x, weight, bias, eps, want_stats):
     affine = _ln_check(x, weight, bias)
-    width = x.shape[-1]
+    width, dev = x.shape[-1], x.device
     xr, rows, stride = _rows(x, width)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty_like(xr, memory_format=torch.contiguous_format)
     mean = rstd = None
     if want_stats:
-        stats = torch.empty((2,) + x.shape[:-1], dtype=F32, device=x.device)
-        mean, rstd = stats[0], stats[1]
-    weight = weight if weight is None else weight.contiguous()
-    bias = bias if bias is None else bias.contiguous()
-    with device_guard(x.device), _timed("layer_norm_forward", rows):
-        check(lib.nsr_layer_norm_forward(xr.data_ptr(), stride, ptr(weight), ptr(bias), y.data_ptr(), ptr(mean), ptr(rstd), rows,
-                                         width, DTYPE_CODES[x.dtype], DTYPE_CODES[affine], float(eps), stream_ptr()),
+        mean = torch.empty(x.shape[:-1], dtype=F32, device=dev)
+        rstd = torch.empty_like(mean)
+    if weight is not None:
+        weight = weight.contiguous()
+    if bias is not None:
+        bias = bias.contiguous()
+    with device_guard(dev), _timed("layer_norm_forward", rows):
+        check(lib.nsr_layer_norm_forward(xr.data_ptr(), stride, _addr(weight), _addr(bias), y.data_ptr(), _addr(mean), _addr(rstd),
+                                         rows, width, DTYPE_CODES[x.dtype], DTYPE_CODES[affine], eps, stream_ptr()),
               "nsr_layer_norm_forward")
     return y, mean, rstd
 
@@ -907,17 +913,20 @@ def layer_norm_backward(dy, x, weight, mean, rstd, want_dx=True, want_dweight=Tr
     width, dev = x.shape[-1], x.device
     xr, rows, stride = _rows(x, width)
     dr, _, dstride = _rows(dy, width)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_dx else None
+    dx = torch.empty_like(xr, memory_format=torch.contiguous_format) if want_dx else None
     dweight = torch.empty(width, dtype=affine, device=dev) if want_dweight else None
     dbias = torch.empty(width, dtype=affine, device=dev) if want_dbias else None
-    ws = None
+    ws, code = None, DTYPE_CODES[x.dtype]
     if want_dweight or want_dbias:
-        ws = torch.empty(lib.nsr_layer_norm_backward_workspace_floats(rows, width, DTYPE_CODES[x.dtype]), dtype=F32, device=dev)
-    weight = weight if weight is None else weight.contiguous()
+        floats = lib.nsr_layer_norm_backward_workspace_floats(rows, width, code)
+        if floats:
+            ws = torch.empty(floats, dtype=F32, device=dev)
+    if weight is not None:
+        weight = weight.contiguous()
     mean, rstd = mean.contiguous(), rstd.contiguous()
     with device_guard(dev), _timed("layer_norm_backward", rows):
-        check(lib.nsr_layer_norm_backward(dr.data_ptr(), dstride, xr.data_ptr(), stride, ptr(weight), ptr(mean), ptr(rstd), ptr(dx),
-                                          ptr(dweight), ptr(dbias), ptr(ws), rows, width, DTYPE_CODES[x.dtype],
+        check(lib.nsr_layer_norm_backward(dr.data_ptr(), dstride, xr.data_ptr(), stride, _addr(weight), mean.data_ptr(),
+                                          rstd.data_ptr(), _addr(dx), _addr(dweight), _addr(dbias), _addr(ws), rows, width, code,
                                           DTYPE_CODES[affine], stream_ptr()), "nsr_layer_norm_backward")
     return dx, dweight, dbias
 
