@@ -3,11 +3,11 @@
 //   dx = s (g - mean(g) - h mean(g h)) with g = dy w,  dw = sum over rows of dy h,  db = sum over rows of dy
 // Statistics, sums and products in fp32 whatever the storage type; the variance from centred values.
 //
-// Bound by HBM: each input is read once, each output written once.  A row is held in registers by a group of G lanes (1 .. 64 in
-// a wave, 256 or 1024 threads above), ITER vectors of 16 bytes a lane, so statistics and result come from one read.  G is the
-// power of two that covers the row: rows of 64 halfs take 8 lanes and a wave works on 8 of them at once (one row per wave would
-// leave 7 of 8 lanes idle).  Vectors are loaded and stored at element alignment (global memory takes any), so odd widths,
-// strides and addresses go the same way; only the vector that a row's end cuts is taken element by element.
+// Bound by HBM: each input is read once, each output written once.  A row is held in registers by a group of G lanes, ITER
+// vectors of 16 bytes a lane, so statistics and result come from one read.  G is the power of two that covers the row, 1 .. 64
+// lanes of a wave, 128 .. 1024 threads above: rows of 64 halfs take 8 lanes and a wave works on 8 of them at once (one row per
+// wave would leave 7 of 8 lanes idle).  Odd widths: the vector at a row's end starts early enough to be whole, what it repeats
+// of the one before counts in no sum and is stored twice with the same value.
 // The backward pass walks rows with the lane's columns fixed: their dw and db sums stay in registers over all rows of a
 // workgroup, go through LDS once and to memory as one row of partial sums per workgroup, which a second launch adds in a fixed
 // order (no atomics: the same bits for the same inputs).
@@ -113,6 +113,55 @@ __device__ __forceinline__ void store_vec(T *row, uint32_t col, uint32_t width, 
     }
 }
 
+// Rows at 4-byte addresses and at least a vector wide (all of fp32 from width 4 on, 16-bit rows of even widths and strides) go
+// through buffer instructions instead: lanes outside the row and rows past the end have offsets past the buffer's end, where
+// loads give zero and stores do nothing.  Nothing then branches around a memory instruction, and only so can the compiler count
+// what is outstanding: behind a branch it waits for everything, also for the loads of the next tile and the stores of the last
+// one (backward, 131072 x 256 bf16: 47.7 us with branches, 41.8 without; 8192 x 4096 bf16, both directions: 86.5 and 72.9 us).
+constexpr uint32_t OUTSIDE = 0x80000000u, BUFFER_MOST = 0x7ffffff0u;
+
+// `left` rows of `row_bytes`, `stride_bytes` apart, from p on (the same values in every lane)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const void *p, int64_t left, uint64_t stride_bytes, uint32_t row_bytes)
+{
+    const uint64_t bytes = left > 0 ? (uint64_t)(left - 1) * stride_bytes + row_bytes : 0;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, (int)(bytes < BUFFER_MOST ? bytes : BUFFER_MOST), 0x00020000);
+}
+
+template <class V>
+__device__ __forceinline__ V buffer_load(__amdgpu_buffer_rsrc_t r, uint32_t offset)
+{
+    V v;
+    if constexpr (sizeof(V) == 16) {
+        const auto u = __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, 0);
+        __builtin_memcpy(&v, &u, 16);
+    } else {
+        const auto u = __builtin_amdgcn_raw_buffer_load_b32(r, offset, 0, 0);
+        __builtin_memcpy(&v, &u, 4);
+    }
+    return v;
+}
+
+template <class V>
+__device__ __forceinline__ void buffer_store(__amdgpu_buffer_rsrc_t r, uint32_t offset, const V &v)
+{
+    static_assert(sizeof(V) == 16, "");
+    decltype(__builtin_amdgcn_raw_buffer_load_b128(r, 0, 0, 0)) u;
+    __builtin_memcpy(&u, &v, 16);
+    __builtin_amdgcn_raw_buffer_store_b128(u, r, offset, 0, 0);
+}
+
+// where vector `i` of a lane lies: its first column, and how many of its elements the vector before holds too (all of them, or
+// more: a lane outside the row)
+struct Place { uint32_t at, twice; };
+template <int N, bool BUFFER>
+__device__ __forceinline__ Place place(uint32_t vector, uint32_t width)
+{
+    const uint32_t col = vector * N;
+    if constexpr (!BUFFER) return {col, 0};
+    const uint32_t at = col + N <= width ? col : width - N;
+    return {at, col - at};
+}
+
 // N affine parameters from `col` on, fp32 or of the rows' type; `none` where there are none
 template <class T, int N>
 __device__ __forceinline__ void load_affine(const void *p, bool fp32, uint32_t col, uint32_t width, float none, float (&v)[N])
@@ -134,8 +183,9 @@ __device__ __forceinline__ void load_affine(const void *p, bool fp32, uint32_t c
 }
 
 // ---- forward ---------------------------------------------------------------------------------------------------------------
-// U rows of each group are loaded before the first is worked on; a lane's weight and bias stay in registers
-template <class T, int G, int ITER, int U>
+// A lane's weight and bias stay in registers.  Groups of more than a wave load the next row while they work on one; smaller ones
+// have enough waves without (2097152 x 64 fp16: 94 us without, 101 us with).
+template <class T, int G, int ITER, bool BUFFER>
 __global__ void __launch_bounds__(G > 256 ? G : 256)
 k_ln_forward(const T *__restrict__ x, uint64_t xs, const void *__restrict__ w, const void *__restrict__ b, int affine_fp32,
              T *__restrict__ y, float *__restrict__ mean, float *__restrict__ rstd, uint64_t rows, uint32_t width,
@@ -145,58 +195,66 @@ k_ln_forward(const T *__restrict__ x, uint64_t xs, const void *__restrict__ w, c
     __shared__ float lds[G > 64 ? 32 : 1];
     int turn = 0;
     const uint32_t lane = threadIdx.x % G, group = threadIdx.x / G;
-    const bool whole = width == (uint32_t)(G * N * ITER);
+    const bool covered = width == (uint32_t)(G * N * ITER);
+    Vec<T, N> raw[ITER];
+    auto load_row = [&](uint64_t tile) {
+        const uint64_t row0 = tile * GROUPS, row = row0 + group;
+        const auto from = rows_buffer(x + row0 * xs, (int64_t)(rows - row0), xs * sizeof(T), width * sizeof(T));
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            const Place p = place<N, BUFFER>(i * G + lane, width);
+            if constexpr (BUFFER) raw[i] = buffer_load<Vec<T, N>>(from, p.twice < N ? (group * (uint32_t)xs + p.at) * sizeof(T) : OUTSIDE);
+            else raw[i] = load_vec(x + row * xs, p.at, row < rows ? width : 0);
+        }
+    };
+    load_row(blockIdx.x);
     float wv[ITER][N], bv[ITER][N];
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
-        load_affine<T>(w, affine_fp32, (i * G + lane) * N, width, 1.f, wv[i]);
-        load_affine<T>(b, affine_fp32, (i * G + lane) * N, width, 0.f, bv[i]);
+        const Place p = place<N, BUFFER>(i * G + lane, width);
+        load_affine<T>(w, affine_fp32, p.at, width, 1.f, wv[i]);
+        load_affine<T>(b, affine_fp32, p.at, width, 0.f, bv[i]);
     }
-    for (uint64_t tile = blockIdx.x; tile * (GROUPS * U) < rows; tile += gridDim.x) {
-        const uint64_t row0 = tile * (GROUPS * U) + group;
-        Vec<T, N> raw[U][ITER];
+    // whether element k of vector i counts in the sums
+    auto counts = [&](int i, int k) {
+        const Place p = place<N, BUFFER>(i * G + lane, width);
+        return k >= (int)p.twice && p.at + k < width;
+    };
+    for (uint64_t tile = blockIdx.x; tile * GROUPS < rows; tile += gridDim.x) {
+        const uint64_t row0 = tile * GROUPS, row = row0 + group;
+        float v[ITER][N], t[1] = {0.f};
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const uint64_t row = row0 + u * GROUPS;
+        for (int i = 0; i < ITER; ++i) {
 #pragma unroll
-            for (int i = 0; i < ITER; ++i) raw[u][i] = load_vec(x + row * xs, (i * G + lane) * N, row < rows ? width : 0);
+            for (int k = 0; k < N; ++k) v[i][k] = (float)raw[i].e[k];
+            if (covered) t[0] += pairwise<N>([&](int k) { return v[i][k]; });
+            else t[0] += pairwise<N>([&](int k) { return counts(i, k) ? v[i][k] : 0.f; });
         }
+        if constexpr (G > 64) load_row(tile + gridDim.x);
+        group_sum<G>(t, lds, turn);
+        const float mu = t[0] * inv_width;
+        t[0] = 0.f;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const uint64_t row = row0 + u * GROUPS;
-            float v[ITER][N], t[1] = {0.f};
+        for (int i = 0; i < ITER; ++i) {
 #pragma unroll
-            for (int i = 0; i < ITER; ++i) {
-#pragma unroll
-                for (int k = 0; k < N; ++k) v[i][k] = (float)raw[u][i].e[k];
-                t[0] += pairwise<N>([&](int k) { return v[i][k]; });
-            }
-            group_sum<G>(t, lds, turn);
-            const float mu = t[0] * inv_width;
-            t[0] = 0.f;
-#pragma unroll
-            for (int i = 0; i < ITER; ++i) {
-#pragma unroll
-                for (int k = 0; k < N; ++k) {
-                    v[i][k] -= mu;
-                    if (!whole && (i * G + lane) * N + k >= width) v[i][k] = 0.f;
-                }
-                t[0] += pairwise<N>([&](int k) { return v[i][k] * v[i][k]; });
-            }
-            group_sum<G>(t, lds, turn);
-            const float rs = 1.f / sqrtf(t[0] * inv_width + eps);
-            if (row < rows) {
-#pragma unroll
-                for (int i = 0; i < ITER; ++i) {
-                    const uint32_t col = (i * G + lane) * N;
-                    Vec<T, N> o;
-#pragma unroll
-                    for (int k = 0; k < N; ++k) o.e[k] = (T)fmaf(v[i][k] * rs, wv[i][k], bv[i][k]);
-                    store_vec(y + row * width, col, width, o);
-                }
-                if (mean && lane == 0) { mean[row] = mu; rstd[row] = rs; }
-            }
+            for (int k = 0; k < N; ++k) v[i][k] -= mu;
+            if (covered) t[0] += pairwise<N>([&](int k) { return v[i][k] * v[i][k]; });
+            else t[0] += pairwise<N>([&](int k) { return counts(i, k) ? v[i][k] * v[i][k] : 0.f; });
         }
+        group_sum<G>(t, lds, turn);
+        const float rs = 1.f / sqrtf(t[0] * inv_width + eps);
+        const auto to = rows_buffer(y + row0 * width, (int64_t)(rows - row0), width * sizeof(T), width * sizeof(T));
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            const Place p = place<N, BUFFER>(i * G + lane, width);
+            Vec<T, N> o;
+#pragma unroll
+            for (int k = 0; k < N; ++k) o.e[k] = (T)fmaf(v[i][k] * rs, wv[i][k], bv[i][k]);
+            if constexpr (BUFFER) buffer_store(to, p.twice < N ? (group * width + p.at) * sizeof(T) : OUTSIDE, o);
+            else if (row < rows) store_vec(y + row * width, p.at, width, o);
+        }
+        if (mean && lane == 0 && row < rows) { mean[row] = mu; rstd[row] = rs; }
+        if constexpr (G <= 64) load_row(tile + gridDim.x);
     }
 }
 
@@ -256,74 +314,102 @@ __device__ __forceinline__ void store_sum(int which, uint32_t col, float v, uint
     }
 }
 
-template <class T, int G, int ITER, int U>
+// The next row of each group is under way as soon as this one is in fp32 registers.  (Two rows ahead: 43.8 instead of 41.1 us
+// for 262144 x 64 fp32, 44.6 instead of 41.8 us for 131072 x 256 bf16.)
+template <class T, int G, int ITER, bool BUFFER>
 __global__ void __launch_bounds__(BWD_THREADS)
 k_ln_backward(const T *__restrict__ dy, uint64_t dys, const T *__restrict__ x, uint64_t xs, const void *__restrict__ w,
               int affine_fp32, const float *__restrict__ mean, const float *__restrict__ rstd, T *__restrict__ dx, void *dw,
               void *db, float *__restrict__ part, uint64_t rows, uint32_t width, float inv_width)
 {
     constexpr int N = Vec16<T>::N, GROUPS = BWD_THREADS / G;
-    // sums: the groups of a wave are added by lane moves first, so LDS holds one row of G ITER N columns per wave or group
+    // sums: the groups of a wave are added by lane moves first, so LDS holds one row of G N columns per wave or group
     constexpr int SETS = G < 64 ? BWD_THREADS / 64 : GROUPS;
     __shared__ float lds[G > 64 ? 64 : 1];
     __shared__ float sums[SETS > 1 ? SETS * G * N : 1];
     int turn = 0;
     const uint32_t lane = threadIdx.x % G, group = threadIdx.x / G;
+    const bool whole = width % N == 0;  // (no element is held twice; what lies outside the row is zero in dy)
+    Vec<T, N> xr[ITER], dr[ITER];
+    float mu, rs;
+    auto load_row = [&](uint64_t tile) {
+        const uint64_t row0 = tile * GROUPS, row = row0 + group;
+        const int64_t left = (int64_t)(rows - row0);
+        const auto from_x = rows_buffer(x + row0 * xs, left, xs * sizeof(T), width * sizeof(T));
+        const auto from_d = rows_buffer(dy + row0 * dys, left, dys * sizeof(T), width * sizeof(T));
+        const uint32_t live = row < rows ? width : 0;
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            const Place p = place<N, BUFFER>(i * G + lane, width);
+            if constexpr (BUFFER) {
+                xr[i] = buffer_load<Vec<T, N>>(from_x, p.twice < N ? (group * (uint32_t)xs + p.at) * sizeof(T) : OUTSIDE);
+                dr[i] = buffer_load<Vec<T, N>>(from_d, p.twice < N ? (group * (uint32_t)dys + p.at) * sizeof(T) : OUTSIDE);
+            } else {
+                xr[i] = load_vec(x + row * xs, p.at, live);
+                dr[i] = load_vec(dy + row * dys, p.at, live);
+            }
+        }
+        mu = buffer_load<float>(rows_buffer(mean + row0, left, 4, 4), group * 4);
+        rs = buffer_load<float>(rows_buffer(rstd + row0, left, 4, 4), group * 4);
+    };
+    load_row(blockIdx.x);
     float wv[ITER][N], sw[ITER][N], sb[ITER][N];
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
-        load_affine<T>(w, affine_fp32, (i * G + lane) * N, width, 1.f, wv[i]);
+        load_affine<T>(w, affine_fp32, place<N, BUFFER>(i * G + lane, width).at, width, 1.f, wv[i]);
 #pragma unroll
         for (int k = 0; k < N; ++k) sw[i][k] = sb[i][k] = 0.f;
     }
-    for (uint64_t tile = blockIdx.x; tile * (GROUPS * U) < rows; tile += gridDim.x) {
-        const uint64_t row0 = tile * (GROUPS * U) + group;
-        Vec<T, N> xr[U][ITER], dr[U][ITER];
-        float mu[U], rs[U];
+    for (uint64_t tile = blockIdx.x; tile * GROUPS < rows; tile += gridDim.x) {
+        const uint64_t row0 = tile * GROUPS, row = row0 + group;
+        float h[ITER][N], g[ITER][N], t[2] = {0.f, 0.f};
+        const float rs0 = rs;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const uint64_t row = row0 + u * GROUPS;
-            const uint32_t live = row < rows ? width : 0;  // (what lies outside is zero: it adds nothing to any sum)
+        for (int i = 0; i < ITER; ++i)
 #pragma unroll
-            for (int i = 0; i < ITER; ++i) {
-                xr[u][i] = load_vec(x + row * xs, (i * G + lane) * N, live);
-                dr[u][i] = load_vec(dy + row * dys, (i * G + lane) * N, live);
+            for (int k = 0; k < N; ++k) {
+                g[i][k] = (float)dr[i].e[k];
+                h[i][k] = ((float)xr[i].e[k] - mu) * rs0;
             }
-            mu[u] = live ? mean[row] : 0.f;
-            rs[u] = live ? rstd[row] : 0.f;
-        }
+        load_row(tile + gridDim.x);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const uint64_t row = row0 + u * GROUPS;
-            float h[ITER][N], g[ITER][N], t[2] = {0.f, 0.f};
+        for (int i = 0; i < ITER; ++i) {
 #pragma unroll
-            for (int i = 0; i < ITER; ++i) {
-#pragma unroll
-                for (int k = 0; k < N; ++k) {
-                    const float d = (float)dr[u][i].e[k];
-                    h[i][k] = ((float)xr[u][i].e[k] - mu[u]) * rs[u];
-                    g[i][k] = d * wv[i][k];
-                    sw[i][k] = fmaf(d, h[i][k], sw[i][k]);
-                    sb[i][k] += d;
-                }
+            for (int k = 0; k < N; ++k) {
+                sw[i][k] = fmaf(g[i][k], h[i][k], sw[i][k]);
+                sb[i][k] += g[i][k];
+                g[i][k] *= wv[i][k];
+            }
+            if (!BUFFER || whole) {
                 t[0] += pairwise<N>([&](int k) { return g[i][k]; });
                 t[1] += pairwise<N>([&](int k) { return g[i][k] * h[i][k]; });
+            } else {
+                const int twice = (int)place<N, BUFFER>(i * G + lane, width).twice;
+                t[0] += pairwise<N>([&](int k) { return k >= twice ? g[i][k] : 0.f; });
+                t[1] += pairwise<N>([&](int k) { return k >= twice ? g[i][k] * h[i][k] : 0.f; });
             }
-            if (dx) {  // (the same for every thread)
-                group_sum<G>(t, lds, turn);
-                const float a = t[0] * inv_width, c = t[1] * inv_width;
-                if (row < rows)
+        }
+        if (dx) {  // (the same for every thread)
+            group_sum<G>(t, lds, turn);
+            const float a = t[0] * inv_width, c = t[1] * inv_width;
+            const auto to = rows_buffer(dx + row0 * width, (int64_t)(rows - row0), width * sizeof(T), width * sizeof(T));
 #pragma unroll
-                    for (int i = 0; i < ITER; ++i) {
-                        Vec<T, N> o;
+            for (int i = 0; i < ITER; ++i) {
+                const Place p = place<N, BUFFER>(i * G + lane, width);
+                Vec<T, N> o;
 #pragma unroll
-                        for (int k = 0; k < N; ++k) o.e[k] = (T)(rs[u] * (g[i][k] - a - h[i][k] * c));
-                        store_vec(dx + row * width, (i * G + lane) * N, width, o);
-                    }
+                for (int k = 0; k < N; ++k) o.e[k] = (T)(rs0 * (g[i][k] - a - h[i][k] * c));
+                if constexpr (BUFFER) buffer_store(to, p.twice < N ? (group * width + p.at) * sizeof(T) : OUTSIDE, o);
+                else if (row < rows) store_vec(dx + row * width, p.at, width, o);
             }
         }
     }
     if (!dw && !db) return;
+    // the sum of element k of vector i of a lane is a column's where it counts
+    auto put_sum = [&](int which, int i, uint32_t of_lane, int k, float v) {
+        const Place p = place<N, BUFFER>(i * G + of_lane, width);
+        if (k >= (int)p.twice && p.at + k < width) store_sum<T>(which, p.at + k, v, width, part, dw, db, affine_fp32);
+    };
 #pragma unroll
     for (int i = 0; i < ITER; ++i)
 #pragma unroll
@@ -331,8 +417,7 @@ k_ln_backward(const T *__restrict__ dy, uint64_t dys, const T *__restrict__ x, u
             float(&s)[N] = which ? sb[i] : sw[i];
             if constexpr (SETS == 1) {
 #pragma unroll
-                for (int k = 0; k < N; ++k)
-                    if ((i * G + lane) * N + k < width) store_sum<T>(which, (i * G + lane) * N + k, s[k], width, part, dw, db, affine_fp32);
+                for (int k = 0; k < N; ++k) put_sum(which, i, lane, k, s[k]);
             } else {
 #pragma unroll
                 for (int k = 0; k < N; ++k)
@@ -345,10 +430,9 @@ k_ln_backward(const T *__restrict__ dy, uint64_t dys, const T *__restrict__ x, u
                     for (int k = 0; k < N; ++k) sums[(set * N + k) * G + lane] = s[k];
                 __syncthreads();
                 for (uint32_t c = threadIdx.x; c < (uint32_t)(G * N); c += BWD_THREADS) {  // c = k G + lane
-                    const uint32_t col = (i * G + c % G) * N + c / G;
                     float v = sums[c];
                     for (int q = 1; q < SETS; ++q) v += sums[q * (G * N) + c];
-                    if (col < width) store_sum<T>(which, col, v, width, part, dw, db, affine_fp32);
+                    put_sum(which, i, c % G, c / G, v);
                 }
             }
         }
@@ -478,27 +562,35 @@ int narrow_group(uint32_t width, F f)
     return f(Int<64>{});
 }
 
-// f(G, ITER): at most 16 columns a lane in the forward pass.  In the backward pass each column has a weight, two sums and two
-// inputs in registers: 16 in groups of up to 256, 8 where 1024 threads share the registers of a CU.
-constexpr uint32_t FORWARD_MOST = 16384, BACKWARD_MOST = 8192;
+// f(G, ITER) for rows of `width`: 1 vector a lane up to a wave, PER columns a lane above it, the smallest G that covers the row.
+constexpr uint32_t FORWARD_COLUMNS = 16, BACKWARD_COLUMNS = 8;
 
-template <class T, uint32_t MOST, class F>
+template <class T, uint32_t PER, class F>
 int row_shape(uint32_t width, F f)
 {
     constexpr uint32_t N = Vec16<T>::N;
+    constexpr int ITER = PER / N;
     if (width <= 64 * N) return narrow_group<(int)N>(width, [&](auto g) { return f(g, Int<1>{}); });
-    if (width <= 128 * N) return f(Int<64>{}, Int<2>{});
-    if (width <= 256 * N) return f(Int<256>{}, Int<1>{});
-    if (width <= 512 * N) return f(Int<256>{}, Int<2>{});
-    if constexpr (MOST >= 1024 * N)
-        if (width <= 1024 * N) return f(Int<1024>{}, Int<1>{});
-    if constexpr (MOST >= 2048 * N)
-        if (width <= 2048 * N) return f(Int<1024>{}, Int<2>{});
-    return f(Int<1024>{}, Int<MOST / (1024 * N)>{});
+    if constexpr (ITER == 4)
+        if (width <= 128 * N) return f(Int<64>{}, Int<2>{});
+    if (width <= 64 * PER) return f(Int<64>{}, Int<ITER>{});
+    if (width <= 128 * PER) return f(Int<128>{}, Int<ITER>{});
+    if (width <= 256 * PER) return f(Int<256>{}, Int<ITER>{});
+    if (width <= 512 * PER) return f(Int<512>{}, Int<ITER>{});
+    return f(Int<1024>{}, Int<ITER>{});
 }
 
-// rows of each group that are in flight at once
-constexpr int rows_at_once(int iter) { return iter == 1 ? 2 : 1; }
+constexpr uint32_t FORWARD_MOST = 1024 * FORWARD_COLUMNS, BACKWARD_MOST = 1024 * BACKWARD_COLUMNS;
+
+// whether rows take buffer instructions: a vector wide, at 4-byte addresses, and `together` of them within the reach of 31-bit
+// offsets
+bool by_buffer(uint32_t width, uint32_t dtype, const void *a, uint64_t as, const void *b, uint64_t bs, const void *c, uint64_t cs,
+               uint32_t together)
+{
+    const uint64_t size = dtype_size(dtype), most = as > bs ? (as > cs ? as : cs) : (bs > cs ? bs : cs);
+    return width * size >= 16 && most < (1ull << 30) && most * size * together < BUFFER_MOST / 2 &&
+           (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c | as * size | bs * size | cs * size) & 3) == 0;
+}
 
 // workgroups of the backward pass = rows of partial sums
 uint32_t backward_groups(uint64_t rows, uint32_t width, uint32_t dtype)
@@ -507,12 +599,12 @@ uint32_t backward_groups(uint64_t rows, uint32_t width, uint32_t dtype)
     uint64_t per = 1;
     if (width <= BACKWARD_MOST)
         ln_type(dtype, [&](auto t) {
-            return row_shape<decltype(t), BACKWARD_MOST>(width, [&](auto g, auto iter) {
-                per = BWD_THREADS / decltype(g)::value * rows_at_once(decltype(iter)::value);
+            return row_shape<decltype(t), BACKWARD_COLUMNS>(width, [&](auto g, auto) {
+                per = BWD_THREADS / decltype(g)::value;
                 return 0;
             });
         });
-    const uint64_t tiles = (rows + per - 1) / per, most = 2 * CUS;
+    const uint64_t tiles = (rows + per - 1) / per, most = CUS;
     return (uint32_t)(tiles < most ? tiles : most);
 }
 
@@ -534,6 +626,7 @@ extern "C" int nsr_layer_norm_forward(const void *x, uint64_t x_stride, const vo
                 "nsr_layer_norm_forward: misaligned pointer");
     const int fp32 = affine_dtype == DT_F32;
     const float inv = 1.f / (float)width;
+    if (rows == 1) x_stride = width;  // (a single row has no stride: the kernels tell rows outside by theirs)
     return ln_type(dtype, [&](auto t) {
         using T = decltype(t);
         if (width > FORWARD_MOST) {
@@ -543,13 +636,14 @@ extern "C" int nsr_layer_norm_forward(const void *x, uint64_t x_stride, const vo
             NSR_CHECK_LAUNCH("nsr_layer_norm_forward");
             return NSR_OK;
         }
-        return row_shape<T, FORWARD_MOST>(width, [&](auto g, auto iter) {
-            constexpr int G = decltype(g)::value, ITER = decltype(iter)::value, U = rows_at_once(ITER);
+        return row_shape<T, FORWARD_COLUMNS>(width, [&](auto g, auto iter) {
+            constexpr int G = decltype(g)::value, ITER = decltype(iter)::value;
             constexpr int THREADS = G > 256 ? G : 256;
-            const uint64_t tiles = (rows + THREADS / G * U - 1) / (THREADS / G * U), most = 8 * CUS * 256 / THREADS;
-            hipLaunchKernelGGL((k_ln_forward<T, G, ITER, U>), dim3((uint32_t)(tiles < most ? tiles : most)), dim3(THREADS), 0,
-                               (hipStream_t)stream, (const T *)x, x_stride, weight, bias, fp32, (T *)y, mean, rstd, rows, width,
-                               inv, eps);
+            const uint64_t tiles = (rows + THREADS / G - 1) / (THREADS / G), most = G <= 64 ? 64 * CUS : 6 * CUS * 256 / THREADS;
+            const bool buffer = by_buffer(width, dtype, x, x_stride, y, width, x, x_stride, THREADS / G);
+            auto kernel = buffer ? k_ln_forward<T, G, ITER, true> : k_ln_forward<T, G, ITER, false>;
+            hipLaunchKernelGGL(kernel, dim3((uint32_t)(tiles < most ? tiles : most)), dim3(THREADS), 0, (hipStream_t)stream,
+                               (const T *)x, x_stride, weight, bias, fp32, (T *)y, mean, rstd, rows, width, inv, eps);
             NSR_CHECK_LAUNCH("nsr_layer_norm_forward");
             return NSR_OK;
         });
@@ -582,13 +676,16 @@ extern "C" int nsr_layer_norm_backward(const void *dy, uint64_t dy_stride, const
     if (!affine && !(dx && rows)) return NSR_OK;
     const int fp32 = affine_dtype == DT_F32;
     const float inv = 1.f / (float)width;
+    if (rows == 1) x_stride = dy_stride = width;  // (a single row has no stride: the kernels tell rows outside by theirs)
     hipStream_t st = (hipStream_t)stream;
     return ln_type(dtype, [&](auto t) {
         using T = decltype(t);
         if (groups && width <= BACKWARD_MOST) {
-            row_shape<T, BACKWARD_MOST>(width, [&](auto g, auto iter) {
+            row_shape<T, BACKWARD_COLUMNS>(width, [&](auto g, auto iter) {
                 constexpr int G = decltype(g)::value, ITER = decltype(iter)::value;
-                hipLaunchKernelGGL((k_ln_backward<T, G, ITER, rows_at_once(ITER)>), dim3(groups), dim3(BWD_THREADS), 0, st,
+                const bool buffer = by_buffer(width, dtype, x, x_stride, dx, width, dy, dy_stride, BWD_THREADS / G);
+                auto kernel = buffer ? k_ln_backward<T, G, ITER, true> : k_ln_backward<T, G, ITER, false>;
+                hipLaunchKernelGGL(kernel, dim3(groups), dim3(BWD_THREADS), 0, st,
                                    (const T *)dy, dy_stride, (const T *)x, x_stride, weight, fp32, mean, rstd, (T *)dx, dweight,
                                    dbias, workspace, rows, width, inv);
                 return 0;

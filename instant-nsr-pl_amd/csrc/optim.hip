@@ -24,8 +24,11 @@ constexpr int OPT_BLOCK = 256;          // elements under one scale: one wave, 4
 // every size (12.6 M fp32 parameters, 32 bits: 68.8 / 70.8 / 76.1 us; 8 bits: 42.2 / 43.9 / 54.1 us): more workgroups hide
 // more latency than more loads in flight in each.
 constexpr int OPT_CHUNK = OPT_THREADS * 4;
-constexpr int NORM_CHUNK = 8192;        // of the gradient norm: 8 (fp32) or 4 (16 bits) vectors a lane in flight
-constexpr uint32_t NORM_MAX_GRID = 1024;  // partial sums per launch of the gradient norm
+// Of the gradient norm: 4 (fp32) or 2 (16 bits) vectors a lane in flight, one or few chunks a workgroup, a partial sum for each
+// workgroup (27.9 M fp32 gradients: 28 us; chunks of 8192 in at most 1024 workgroups 33 us, 2048 in 8192 as fast but twice the
+// sums to add).
+constexpr int NORM_CHUNK = 4096;
+constexpr uint32_t NORM_MAX_GRID = 4096;  // partial sums per launch
 constexpr float E4M3_TOP = 448.f, E4M3_INV_TOP = 1.f / 448.f;
 constexpr float LEAST_TOP = 7.888609052210118e-31f;    // 2^-100: keeps 448 / top and top / 448 normal numbers
 constexpr float ROOT_MOST = 1.8446743e19f;             // sqrt of the largest float: a root stays finite in 8 bits
@@ -89,7 +92,8 @@ __device__ __forceinline__ void adamw_elem(float &p, float &m, float &v, float g
     m = take ? m1 : m;
     v = take ? v1 : v;
     r = sqrtf(v);
-    const float p1 = p * s.decay - s.step * (m / (r * s.root + s.eps));
+    // (the reciprocal instruction is good to 1 ulp, of an update that is a small part of p; the division cost the 8-bit form 4 %)
+    const float p1 = p * s.decay - s.step * (m * __builtin_amdgcn_rcpf(r * s.root + s.eps));
     p = take ? p1 : p;
 }
 
@@ -114,12 +118,15 @@ __device__ __forceinline__ uint32_t e4m3_stochastic(float y, uint32_t bits16)
 __device__ __forceinline__ float wave_max_nonnegative(float v)  // (bits of non-negative floats are ordered like the floats)
 {
     uint32_t x = __float_as_uint(v);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const uint32_t y = (uint32_t)__shfl_xor((int)x, o, 64);
-        x = y > x ? y : x;
-    }
-    return __uint_as_float(x);
+    auto up = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+    x = up(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xf, 0xf, true));   // quad_perm 1 0 3 2
+    x = up(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xf, 0xf, true));   // quad_perm 2 3 0 1
+    x = up(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x141, 0xf, 0xf, true));  // row_half_mirror
+    x = up(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x140, 0xf, 0xf, true));  // row_mirror
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = up(r[0], r[1]);
+    const auto q = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return __uint_as_float(up(q[0], q[1]));
 }
 
 __device__ __forceinline__ float e4m3_value(uint32_t code) { return __builtin_amdgcn_cvt_f32_fp8((int)code, 0); }
@@ -329,20 +336,22 @@ __device__ __forceinline__ double chunk_squares(const void *grad, uint64_t n, ui
     constexpr int N = 16 / sizeof(T), PASSES = NORM_CHUNK / (OPT_THREADS * N);
     const T *g = (const T *)grad + base;
     double acc[2] = {0.0, 0.0};  // (two chains of additions)
-    if (n - base >= NORM_CHUNK) {
-        Vec<T, N> v[PASSES];
+    const uint32_t left = n - base < NORM_CHUNK ? (uint32_t)(n - base) : NORM_CHUNK;
+    Vec<T, N> v[PASSES];
 #pragma unroll
-        for (int it = 0; it < PASSES; ++it) v[it] = get<Vec<T, N>>(g + (it * OPT_THREADS + threadIdx.x) * N);
+    for (int it = 0; it < PASSES; ++it) {
+        const uint32_t i = (it * OPT_THREADS + threadIdx.x) * N;
+        if (i + N <= left) {
+            v[it] = get<Vec<T, N>>(g + i);
+        } else {
 #pragma unroll
-        for (int it = 0; it < PASSES; ++it)
-#pragma unroll
-            for (int k = 0; k < N; ++k) { const double d = (double)(float)v[it].e[k]; acc[k & 1] = fma(d, d, acc[k & 1]); }
-    } else {
-        for (uint32_t i = threadIdx.x; i < (uint32_t)(n - base); i += OPT_THREADS) {
-            const double d = (double)(float)g[i];
-            acc[0] = fma(d, d, acc[0]);
+            for (int k = 0; k < N; ++k) v[it].e[k] = i + k < left ? g[i + k] : (T)0.f;
         }
     }
+#pragma unroll
+    for (int it = 0; it < PASSES; ++it)
+#pragma unroll
+        for (int k = 0; k < N; ++k) { const double d = (double)(float)v[it].e[k]; acc[k & 1] = fma(d, d, acc[k & 1]); }
     return acc[0] + acc[1];
 }
 
