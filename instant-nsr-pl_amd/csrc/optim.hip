@@ -168,7 +168,10 @@ template <class V, class T> __device__ __forceinline__ V get(const T *p)  // (gl
     __builtin_memcpy(&v, p, sizeof(v));
     return v;
 }
-template <class V, class T> __device__ __forceinline__ void put(T *p, const V &v) { __builtin_memcpy(p, &v, sizeof(v)); }
+template <class V, class T> __device__ __forceinline__ void put(T *p, const V &v)
+{
+    __builtin_memcpy(p, &v, sizeof(v));
+}
 
 __device__ __forceinline__ uint32_t random_bits(uint64_t e, uint32_t key0)
 {
@@ -299,10 +302,13 @@ k_adamw_tensors(const Launch<D, MOST> a, OptScalars s, uint32_t seed, uint32_t s
         s.root = hyper[2];
         step = (uint32_t)__float_as_int(hyper[4]);
     }
-    const uint32_t which = tensor_of(a, blockIdx.x);
+    // from the last chunk to the first: the gradients that the norm (or the backward pass) touched last are nearest in the
+    // caches (1 to 2 % for 8-bit moments)
+    const uint32_t chunk = gridDim.x - 1 - blockIdx.x;
+    const uint32_t which = tensor_of(a, chunk);
     const D &t = a.t[which];
     const uint32_t flags = (uint32_t)(t.size >> SIZE_BITS);
-    const uint64_t n = t.size & ((1ull << SIZE_BITS) - 1), base = (uint64_t)(blockIdx.x - a.first[which]) * OPT_CHUNK;
+    const uint64_t n = t.size & ((1ull << SIZE_BITS) - 1), base = (uint64_t)(chunk - a.first[which]) * OPT_CHUNK;
     float lr = t.lr;
     s.decay = t.decay;
     uint32_t key0 = 0;
