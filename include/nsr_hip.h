@@ -1086,7 +1086,8 @@ int nsr_adamw_begin(int32_t *step, float *hyper, double beta1, double beta2, con
 /* ------------------------------------------------------------------------------------------------
  * Layer norm over the last axis, for networks beside the fused 64-wide ones (the reference's VanillaMLP takes any torch layer:
  * models/network_utils.py:100-139).  Types as above; weight and bias (both may be NULL) are fp32 or of the input's type.
- * x and dy have a row stride in elements, y and dx are contiguous.  Statistics and sums in fp32.
+ * x and dy have a row stride in elements (of a single row it is not looked at), y and dx are contiguous and overlap no input.
+ * Statistics and sums in fp32.
  * ------------------------------------------------------------------------------------------------ */
 /* y = (x - mean) * rstd * weight + bias; mean / rstd (float[rows], both or neither) are kept for the backward pass */
 int nsr_layer_norm_forward(const void *x, uint64_t x_stride, const void *weight, const void *bias, void *y, float *mean,

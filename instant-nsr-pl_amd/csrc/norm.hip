@@ -113,11 +113,16 @@ __device__ __forceinline__ void store_vec(T *row, uint32_t col, uint32_t width, 
     }
 }
 
-// Rows at 4-byte addresses and at least a vector wide (all of fp32 from width 4 on, 16-bit rows of even widths and strides) go
-// through buffer instructions instead: lanes outside the row and rows past the end have offsets past the buffer's end, where
-// loads give zero and stores do nothing.  Nothing then branches around a memory instruction, and only so can the compiler count
-// what is outstanding: behind a branch it waits for everything, also for the loads of the next tile and the stores of the last
-// one (backward, 131072 x 256 bf16: 47.7 us with branches, 41.8 without; 8192 x 4096 bf16, both directions: 86.5 and 72.9 us).
+// How a row's vectors are read and written:
+//   BUFFER  rows at 4-byte addresses (fp32; 16 bits with even widths and strides): buffer instructions, where lanes outside the
+//           row and rows past the end have offsets past the buffer's end: loads give zero, stores do nothing;
+//   GLOBAL  16-bit rows at odd addresses: global instructions, which take any address; a lane outside the row repeats its last
+//           vector and a row past the end the last row, which stores what is stored there anyway;
+//   TINY    rows of less than a vector, element by element.
+// In the first two nothing branches around a load, in the first around a store either, and only so can the compiler count what
+// is outstanding: behind a branch it waits for everything, also for the loads of the next row and the stores of the last one
+// (backward, 131072 x 256 bf16: 47.7 us with branches, 41.8 without; 516222 x 65 bf16: 89.9 and 55.4 us).
+enum Access { BUFFER, GLOBAL, TINY };
 constexpr uint32_t OUTSIDE = 0x80000000u, BUFFER_MOST = 0x7ffffff0u;
 
 // `left` rows of `row_bytes`, `stride_bytes` apart, from p on (the same values in every lane)
@@ -144,23 +149,62 @@ __device__ __forceinline__ V buffer_load(__amdgpu_buffer_rsrc_t r, uint32_t offs
 template <class V>
 __device__ __forceinline__ void buffer_store(__amdgpu_buffer_rsrc_t r, uint32_t offset, const V &v)
 {
-    static_assert(sizeof(V) == 16, "");
-    decltype(__builtin_amdgcn_raw_buffer_load_b128(r, 0, 0, 0)) u;
-    __builtin_memcpy(&u, &v, 16);
-    __builtin_amdgcn_raw_buffer_store_b128(u, r, offset, 0, 0);
+    if constexpr (sizeof(V) == 16) {
+        decltype(__builtin_amdgcn_raw_buffer_load_b128(r, 0, 0, 0)) u;
+        __builtin_memcpy(&u, &v, 16);
+        __builtin_amdgcn_raw_buffer_store_b128(u, r, offset, 0, 0);
+    } else {
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), r, offset, 0, 0);
+    }
 }
 
-// where vector `i` of a lane lies: its first column, and how many of its elements the vector before holds too (all of them, or
+// where a vector of the row lies: its first column, and how many of its elements the vector before holds too (all of them, or
 // more: a lane outside the row)
 struct Place { uint32_t at, twice; };
-template <int N, bool BUFFER>
+template <int N, Access A>
 __device__ __forceinline__ Place place(uint32_t vector, uint32_t width)
 {
     const uint32_t col = vector * N;
-    if constexpr (!BUFFER) return {col, 0};
+    if constexpr (A == TINY) return {col, 0};
     const uint32_t at = col + N <= width ? col : width - N;
     return {at, col - at};
 }
+
+// the rows of a tile, row0 .. row0 + groups - 1, in memory
+template <class T, Access A>
+struct Rows {
+    static constexpr int N = Vec16<T>::N;
+    __amdgpu_buffer_rsrc_t buffer;
+    T *row;
+    uint32_t group_at, width;  // (width 0: nothing to read or write, TINY)
+
+    __device__ __forceinline__ Rows(const T *p, uint64_t stride, uint64_t row0, uint32_t group, uint64_t rows, uint32_t width_)
+        : width(width_)
+    {
+        if constexpr (A == BUFFER) {
+            buffer = rows_buffer(p + row0 * stride, (int64_t)(rows - row0), stride * sizeof(T), width_ * sizeof(T));
+            group_at = group * (uint32_t)stride;
+        } else {
+            const uint64_t r = row0 + group;
+            if (A == TINY && r >= rows) width = 0;
+            row = const_cast<T *>(p) + (r < rows ? r : rows - 1) * stride;
+        }
+    }
+    __device__ __forceinline__ Vec<T, N> load(const Place &p) const
+    {
+        if constexpr (A == BUFFER) return buffer_load<Vec<T, N>>(buffer, p.twice < N ? (group_at + p.at) * sizeof(T) : OUTSIDE);
+        if constexpr (A == TINY) return load_vec(row, p.at, width);
+        Vec<T, N> v;
+        __builtin_memcpy(&v, row + p.at, sizeof(v));
+        return v;
+    }
+    __device__ __forceinline__ void store(const Place &p, const Vec<T, N> &v) const
+    {
+        if constexpr (A == BUFFER) buffer_store(buffer, p.twice < N ? (group_at + p.at) * sizeof(T) : OUTSIDE, v);
+        else if constexpr (A == TINY) store_vec(row, p.at, width, v);
+        else if (p.twice < N) __builtin_memcpy(row + p.at, &v, sizeof(v));
+    }
+};
 
 // N affine parameters from `col` on, fp32 or of the rows' type; `none` where there are none
 template <class T, int N>
@@ -185,7 +229,7 @@ __device__ __forceinline__ void load_affine(const void *p, bool fp32, uint32_t c
 // ---- forward ---------------------------------------------------------------------------------------------------------------
 // A lane's weight and bias stay in registers.  Groups of more than a wave load the next row while they work on one; smaller ones
 // have enough waves without (2097152 x 64 fp16: 94 us without, 101 us with).
-template <class T, int G, int ITER, bool BUFFER>
+template <class T, int G, int ITER, Access A>
 __global__ void __launch_bounds__(G > 256 ? G : 256)
 k_ln_forward(const T *__restrict__ x, uint64_t xs, const void *__restrict__ w, const void *__restrict__ b, int affine_fp32,
              T *__restrict__ y, float *__restrict__ mean, float *__restrict__ rstd, uint64_t rows, uint32_t width,
@@ -198,30 +242,26 @@ k_ln_forward(const T *__restrict__ x, uint64_t xs, const void *__restrict__ w, c
     const bool covered = width == (uint32_t)(G * N * ITER);
     Vec<T, N> raw[ITER];
     auto load_row = [&](uint64_t tile) {
-        const uint64_t row0 = tile * GROUPS, row = row0 + group;
-        const auto from = rows_buffer(x + row0 * xs, (int64_t)(rows - row0), xs * sizeof(T), width * sizeof(T));
+        const Rows<T, A> from(x, xs, tile * GROUPS, group, rows, width);
 #pragma unroll
-        for (int i = 0; i < ITER; ++i) {
-            const Place p = place<N, BUFFER>(i * G + lane, width);
-            if constexpr (BUFFER) raw[i] = buffer_load<Vec<T, N>>(from, p.twice < N ? (group * (uint32_t)xs + p.at) * sizeof(T) : OUTSIDE);
-            else raw[i] = load_vec(x + row * xs, p.at, row < rows ? width : 0);
-        }
+        for (int i = 0; i < ITER; ++i) raw[i] = from.load(place<N, A>(i * G + lane, width));
     };
     load_row(blockIdx.x);
     float wv[ITER][N], bv[ITER][N];
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
-        const Place p = place<N, BUFFER>(i * G + lane, width);
+        const Place p = place<N, A>(i * G + lane, width);
         load_affine<T>(w, affine_fp32, p.at, width, 1.f, wv[i]);
         load_affine<T>(b, affine_fp32, p.at, width, 0.f, bv[i]);
     }
     // whether element k of vector i counts in the sums
     auto counts = [&](int i, int k) {
-        const Place p = place<N, BUFFER>(i * G + lane, width);
+        const Place p = place<N, A>(i * G + lane, width);
         return k >= (int)p.twice && p.at + k < width;
     };
     for (uint64_t tile = blockIdx.x; tile * GROUPS < rows; tile += gridDim.x) {
-        const uint64_t row0 = tile * GROUPS, row = row0 + group;
+        const uint64_t row0 = tile * GROUPS;
+        const int64_t left = mean ? (int64_t)(rows - row0) : 0;  // (of the statistics)
         float v[ITER][N], t[1] = {0.f};
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
@@ -243,17 +283,16 @@ k_ln_forward(const T *__restrict__ x, uint64_t xs, const void *__restrict__ w, c
         }
         group_sum<G>(t, lds, turn);
         const float rs = 1.f / sqrtf(t[0] * inv_width + eps);
-        const auto to = rows_buffer(y + row0 * width, (int64_t)(rows - row0), width * sizeof(T), width * sizeof(T));
+        const Rows<T, A> to(y, width, row0, group, rows, width);
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
-            const Place p = place<N, BUFFER>(i * G + lane, width);
             Vec<T, N> o;
 #pragma unroll
             for (int k = 0; k < N; ++k) o.e[k] = (T)fmaf(v[i][k] * rs, wv[i][k], bv[i][k]);
-            if constexpr (BUFFER) buffer_store(to, p.twice < N ? (group * width + p.at) * sizeof(T) : OUTSIDE, o);
-            else if (row < rows) store_vec(y + row * width, p.at, width, o);
+            to.store(place<N, A>(i * G + lane, width), o);
         }
-        if (mean && lane == 0 && row < rows) { mean[row] = mu; rstd[row] = rs; }
+        buffer_store(rows_buffer(mean + row0, left, 4, 4), lane == 0 ? group * 4 : OUTSIDE, mu);
+        buffer_store(rows_buffer(rstd + row0, left, 4, 4), lane == 0 ? group * 4 : OUTSIDE, rs);
         if constexpr (G <= 64) load_row(tile + gridDim.x);
     }
 }
@@ -316,7 +355,7 @@ __device__ __forceinline__ void store_sum(int which, uint32_t col, float v, uint
 
 // The next row of each group is under way as soon as this one is in fp32 registers.  (Two rows ahead: 43.8 instead of 41.1 us
 // for 262144 x 64 fp32, 44.6 instead of 41.8 us for 131072 x 256 bf16.)
-template <class T, int G, int ITER, bool BUFFER>
+template <class T, int G, int ITER, Access A>
 __global__ void __launch_bounds__(BWD_THREADS)
 k_ln_backward(const T *__restrict__ dy, uint64_t dys, const T *__restrict__ x, uint64_t xs, const void *__restrict__ w,
               int affine_fp32, const float *__restrict__ mean, const float *__restrict__ rstd, T *__restrict__ dx, void *dw,
@@ -329,34 +368,36 @@ k_ln_backward(const T *__restrict__ dy, uint64_t dys, const T *__restrict__ x, u
     __shared__ float sums[SETS > 1 ? SETS * G * N : 1];
     int turn = 0;
     const uint32_t lane = threadIdx.x % G, group = threadIdx.x / G;
-    const bool whole = width % N == 0;  // (no element is held twice; what lies outside the row is zero in dy)
+    // no element counts twice: what lies outside the row is zero, or nothing does
+    const bool whole = A == TINY || (A == BUFFER && width % N == 0) || width == (uint32_t)(G * N * ITER);
     Vec<T, N> xr[ITER], dr[ITER];
     float mu, rs;
     auto load_row = [&](uint64_t tile) {
-        const uint64_t row0 = tile * GROUPS, row = row0 + group;
+        const uint64_t row0 = tile * GROUPS;
         const int64_t left = (int64_t)(rows - row0);
-        const auto from_x = rows_buffer(x + row0 * xs, left, xs * sizeof(T), width * sizeof(T));
-        const auto from_d = rows_buffer(dy + row0 * dys, left, dys * sizeof(T), width * sizeof(T));
-        const uint32_t live = row < rows ? width : 0;
+        const Rows<T, A> from_x(x, xs, row0, group, rows, width), from_d(dy, dys, row0, group, rows, width);
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
-            const Place p = place<N, BUFFER>(i * G + lane, width);
-            if constexpr (BUFFER) {
-                xr[i] = buffer_load<Vec<T, N>>(from_x, p.twice < N ? (group * (uint32_t)xs + p.at) * sizeof(T) : OUTSIDE);
-                dr[i] = buffer_load<Vec<T, N>>(from_d, p.twice < N ? (group * (uint32_t)dys + p.at) * sizeof(T) : OUTSIDE);
-            } else {
-                xr[i] = load_vec(x + row * xs, p.at, live);
-                dr[i] = load_vec(dy + row * dys, p.at, live);
-            }
+            const Place p = place<N, A>(i * G + lane, width);
+            xr[i] = from_x.load(p);
+            dr[i] = from_d.load(p);
         }
-        mu = buffer_load<float>(rows_buffer(mean + row0, left, 4, 4), group * 4);
-        rs = buffer_load<float>(rows_buffer(rstd + row0, left, 4, 4), group * 4);
+        if constexpr (A == BUFFER) {
+            mu = buffer_load<float>(rows_buffer(mean + row0, left, 4, 4), group * 4);
+            rs = buffer_load<float>(rows_buffer(rstd + row0, left, 4, 4), group * 4);
+        } else {
+            const uint64_t r = group < left ? row0 + group : rows - 1;
+            mu = mean[r];
+            rs = rstd[r];
+        }
     };
     load_row(blockIdx.x);
-    float wv[ITER][N], sw[ITER][N], sb[ITER][N];
+    // 16 columns a lane leave no registers for the weight, it is read for each row (from the cache); 8 have them
+    constexpr bool HELD = N * ITER <= 8;
+    float wv[HELD ? ITER : 1][N], sw[ITER][N], sb[ITER][N];
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
-        load_affine<T>(w, affine_fp32, place<N, BUFFER>(i * G + lane, width).at, width, 1.f, wv[i]);
+        if constexpr (HELD) load_affine<T>(w, affine_fp32, place<N, A>(i * G + lane, width).at, width, 1.f, wv[i]);
 #pragma unroll
         for (int k = 0; k < N; ++k) sw[i][k] = sb[i][k] = 0.f;
     }
@@ -371,20 +412,26 @@ k_ln_backward(const T *__restrict__ dy, uint64_t dys, const T *__restrict__ x, u
                 g[i][k] = (float)dr[i].e[k];
                 h[i][k] = ((float)xr[i].e[k] - mu) * rs0;
             }
-        load_row(tile + gridDim.x);
+        if constexpr (HELD) load_row(tile + gridDim.x);
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
+            if constexpr (!HELD) {
+                uint32_t at = place<N, A>(i * G + lane, width).at;
+                asm volatile("" : "+v"(at));  // (or the compiler takes the loads out of the loop, and spills)
+                load_affine<T>(w, affine_fp32, at, width, 1.f, wv[0]);
+            }
 #pragma unroll
             for (int k = 0; k < N; ++k) {
-                sw[i][k] = fmaf(g[i][k], h[i][k], sw[i][k]);
-                sb[i][k] += g[i][k];
-                g[i][k] *= wv[i][k];
+                const float d = A == GLOBAL && row >= rows ? 0.f : g[i][k];  // (a row that repeats the last one)
+                sw[i][k] = fmaf(d, h[i][k], sw[i][k]);
+                sb[i][k] += d;
+                g[i][k] *= wv[HELD ? i : 0][k];
             }
-            if (!BUFFER || whole) {
+            if (whole) {
                 t[0] += pairwise<N>([&](int k) { return g[i][k]; });
                 t[1] += pairwise<N>([&](int k) { return g[i][k] * h[i][k]; });
             } else {
-                const int twice = (int)place<N, BUFFER>(i * G + lane, width).twice;
+                const int twice = (int)place<N, A>(i * G + lane, width).twice;
                 t[0] += pairwise<N>([&](int k) { return k >= twice ? g[i][k] : 0.f; });
                 t[1] += pairwise<N>([&](int k) { return k >= twice ? g[i][k] * h[i][k] : 0.f; });
             }
@@ -392,22 +439,21 @@ k_ln_backward(const T *__restrict__ dy, uint64_t dys, const T *__restrict__ x, u
         if (dx) {  // (the same for every thread)
             group_sum<G>(t, lds, turn);
             const float a = t[0] * inv_width, c = t[1] * inv_width;
-            const auto to = rows_buffer(dx + row0 * width, (int64_t)(rows - row0), width * sizeof(T), width * sizeof(T));
+            const Rows<T, A> to(dx, width, row0, group, rows, width);
 #pragma unroll
             for (int i = 0; i < ITER; ++i) {
-                const Place p = place<N, BUFFER>(i * G + lane, width);
                 Vec<T, N> o;
 #pragma unroll
                 for (int k = 0; k < N; ++k) o.e[k] = (T)(rs0 * (g[i][k] - a - h[i][k] * c));
-                if constexpr (BUFFER) buffer_store(to, p.twice < N ? (group * width + p.at) * sizeof(T) : OUTSIDE, o);
-                else if (row < rows) store_vec(dx + row * width, p.at, width, o);
+                to.store(place<N, A>(i * G + lane, width), o);
             }
         }
+        if constexpr (!HELD) load_row(tile + gridDim.x);
     }
     if (!dw && !db) return;
     // the sum of element k of vector i of a lane is a column's where it counts
     auto put_sum = [&](int which, int i, uint32_t of_lane, int k, float v) {
-        const Place p = place<N, BUFFER>(i * G + of_lane, width);
+        const Place p = place<N, A>(i * G + of_lane, width);
         if (k >= (int)p.twice && p.at + k < width) store_sum<T>(which, p.at + k, v, width, part, dw, db, affine_fp32);
     };
 #pragma unroll
@@ -483,23 +529,35 @@ k_ln_backward_long_columns(const T *__restrict__ dy, uint64_t dys, const T *__re
                            void *db, int affine_fp32, uint64_t rows, uint32_t width)
 {
     constexpr int N = Vec16<T>::N;
-    const uint64_t col = ((uint64_t)blockIdx.y * BWD_THREADS + threadIdx.x) * N;
-    if (col >= width) return;
+    const Place p = place<N, GLOBAL>(blockIdx.y * BWD_THREADS + threadIdx.x, width);
+    if (p.twice >= N) return;
     float sw[N] = {}, sb[N] = {};
-    for (uint64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-        const Vec<T, N> xv = load_vec(x + row * xs, (uint32_t)col, width), dv = load_vec(dy + row * dys, (uint32_t)col, width);
-        const float mu = mean[row], rs = rstd[row];
+    for (uint64_t row0 = blockIdx.x; row0 < rows; row0 += 4ull * gridDim.x) {  // four rows under way
+        Vec<T, N> xv[4], dv[4];
+        float mu[4], rs[4];
 #pragma unroll
-        for (int k = 0; k < N; ++k) {
-            sw[k] = fmaf((float)dv.e[k], ((float)xv.e[k] - mu) * rs, sw[k]);
-            sb[k] += (float)dv.e[k];
+        for (int u = 0; u < 4; ++u) {
+            const uint64_t r = row0 + (uint64_t)u * gridDim.x, row = r < rows ? r : rows - 1;
+            __builtin_memcpy(&xv[u], x + row * xs + p.at, sizeof(xv[u]));
+            __builtin_memcpy(&dv[u], dy + row * dys + p.at, sizeof(dv[u]));
+            mu[u] = mean[row];
+            rs[u] = rstd[row];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (row0 + (uint64_t)u * gridDim.x >= rows) break;
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                sw[k] = fmaf((float)dv[u].e[k], ((float)xv[u].e[k] - mu[u]) * rs[u], sw[k]);
+                sb[k] += (float)dv[u].e[k];
+            }
         }
     }
 #pragma unroll
     for (int k = 0; k < N; ++k)
-        if (col + k < width) {
-            store_sum<T>(0, (uint32_t)col + k, sw[k], width, part, dw, db, affine_fp32);
-            store_sum<T>(1, (uint32_t)col + k, sb[k], width, part, dw, db, affine_fp32);
+        if (k >= (int)p.twice) {
+            store_sum<T>(0, p.at + k, sw[k], width, part, dw, db, affine_fp32);
+            store_sum<T>(1, p.at + k, sb[k], width, part, dw, db, affine_fp32);
         }
 }
 
@@ -563,9 +621,10 @@ int narrow_group(uint32_t width, F f)
 }
 
 // f(G, ITER) for rows of `width`: 1 vector a lane up to a wave, 8 columns a lane above it, the smallest G that covers the row.
-// (16 columns a lane of half as large groups: 74 instead of 69 us for both directions of 8192 x 4096 bf16.)  In the backward pass
-// each column has a weight, two sums and two inputs in registers; the forward pass has room for 16 in the widest group.
-constexpr uint32_t BACKWARD_MOST = 8192, FORWARD_MOST = 16384;
+// (16 columns a lane of half as large groups: 74 instead of 69 us for both directions of 8192 x 4096 bf16.)  The widest group
+// takes more, as many as the registers hold: forward 16, backward (two sums and two inputs a column) 16 of 16 bits, 12 of fp32.
+constexpr uint32_t FORWARD_MOST = 16384;
+constexpr uint32_t backward_most(uint32_t dtype) { return dtype == DT_F32 ? 12288 : 16384; }
 
 template <class T, uint32_t MOST, class F>
 int row_shape(uint32_t width, F f)
@@ -577,19 +636,19 @@ int row_shape(uint32_t width, F f)
     if (width <= 128 * 8) return f(Int<128>{}, Int<8 / N>{});
     if (width <= 256 * 8) return f(Int<256>{}, Int<8 / N>{});
     if (width <= 512 * 8) return f(Int<512>{}, Int<8 / N>{});
-    if constexpr (MOST > 1024 * 8)
-        if (width > 1024 * 8) return f(Int<1024>{}, Int<16 / N>{});
-    return f(Int<1024>{}, Int<8 / N>{});
+    if (width <= 1024 * 8) return f(Int<1024>{}, Int<8 / N>{});
+    return f(Int<1024>{}, Int<MOST / (1024 * N)>{});
 }
 
-// whether rows take buffer instructions: a vector wide, at 4-byte addresses, and `together` of them within the reach of 31-bit
-// offsets
-bool by_buffer(uint32_t width, uint32_t dtype, const void *a, uint64_t as, const void *b, uint64_t bs, const void *c, uint64_t cs,
-               uint32_t together)
+// BUFFER needs 4-byte addresses and `together` rows within the reach of 31-bit offsets
+Access access_of(uint32_t width, uint32_t dtype, const void *a, uint64_t as, const void *b, uint64_t bs, const void *c, uint64_t cs,
+                 uint32_t together)
 {
     const uint64_t size = dtype_size(dtype), most = as > bs ? (as > cs ? as : cs) : (bs > cs ? bs : cs);
-    return width * size >= 16 && most < (1ull << 30) && most * size * together < BUFFER_MOST / 2 &&
-           (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c | as * size | bs * size | cs * size) & 3) == 0;
+    if (width * size < 16) return TINY;
+    return most < (1ull << 30) && most * size * together < BUFFER_MOST / 2 &&
+                   (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c | as * size | bs * size | cs * size) & 3) == 0
+               ? BUFFER : GLOBAL;
 }
 
 // workgroups of the backward pass = rows of partial sums
@@ -597,9 +656,9 @@ uint32_t backward_groups(uint64_t rows, uint32_t width, uint32_t dtype)
 {
     if (rows == 0) return 0;
     uint64_t per = 1;
-    if (width <= BACKWARD_MOST)
+    if (width <= backward_most(dtype))
         ln_type(dtype, [&](auto t) {
-            return row_shape<decltype(t), BACKWARD_MOST>(width, [&](auto g, auto) {
+            return row_shape<decltype(t), backward_most(sizeof(t) == 4 ? DT_F32 : DT_F16)>(width, [&](auto g, auto) {
                 per = BWD_THREADS / decltype(g)::value;
                 return 0;
             });
@@ -640,8 +699,10 @@ extern "C" int nsr_layer_norm_forward(const void *x, uint64_t x_stride, const vo
             constexpr int G = decltype(g)::value, ITER = decltype(iter)::value;
             constexpr int THREADS = G > 256 ? G : 256;
             const uint64_t tiles = (rows + THREADS / G - 1) / (THREADS / G), most = G <= 64 ? 64 * CUS : 8 * CUS * 256 / THREADS;
-            const bool buffer = by_buffer(width, dtype, x, x_stride, y, width, x, x_stride, THREADS / G);
-            auto kernel = buffer ? k_ln_forward<T, G, ITER, true> : k_ln_forward<T, G, ITER, false>;
+            const Access access = access_of(width, dtype, x, x_stride, y, width, x, x_stride, THREADS / G);
+            auto kernel = access == BUFFER ? k_ln_forward<T, G, ITER, BUFFER> : k_ln_forward<T, G, ITER, GLOBAL>;
+            if constexpr (G == 1)
+                if (access == TINY) kernel = k_ln_forward<T, G, ITER, TINY>;
             hipLaunchKernelGGL(kernel, dim3((uint32_t)(tiles < most ? tiles : most)), dim3(THREADS), 0, (hipStream_t)stream,
                                (const T *)x, x_stride, weight, bias, fp32, (T *)y, mean, rstd, rows, width, inv, eps);
             NSR_CHECK_LAUNCH("nsr_layer_norm_forward");
@@ -680,11 +741,13 @@ extern "C" int nsr_layer_norm_backward(const void *dy, uint64_t dy_stride, const
     hipStream_t st = (hipStream_t)stream;
     return ln_type(dtype, [&](auto t) {
         using T = decltype(t);
-        if (groups && width <= BACKWARD_MOST) {
-            row_shape<T, BACKWARD_MOST>(width, [&](auto g, auto iter) {
+        if (groups && width <= backward_most(dtype)) {
+            row_shape<T, backward_most(sizeof(T) == 4 ? DT_F32 : DT_F16)>(width, [&](auto g, auto iter) {
                 constexpr int G = decltype(g)::value, ITER = decltype(iter)::value;
-                const bool buffer = by_buffer(width, dtype, x, x_stride, dx, width, dy, dy_stride, BWD_THREADS / G);
-                auto kernel = buffer ? k_ln_backward<T, G, ITER, true> : k_ln_backward<T, G, ITER, false>;
+                const Access access = access_of(width, dtype, x, x_stride, dx, width, dy, dy_stride, BWD_THREADS / G);
+                auto kernel = access == BUFFER ? k_ln_backward<T, G, ITER, BUFFER> : k_ln_backward<T, G, ITER, GLOBAL>;
+                if constexpr (G == 1)
+                    if (access == TINY) kernel = k_ln_backward<T, G, ITER, TINY>;
                 hipLaunchKernelGGL(kernel, dim3(groups), dim3(BWD_THREADS), 0, st,
                                    (const T *)dy, dy_stride, (const T *)x, x_stride, weight, fp32, mean, rstd, (T *)dx, dweight,
                                    dbias, workspace, rows, width, inv);

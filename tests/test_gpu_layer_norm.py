@@ -299,3 +299,55 @@ def test_refusals_on_the_gpu():
                 lambda: ops.layer_norm_backward(dy, x, w, mean.double(), rstd), lambda: ops.layer_norm(x, w, b, -1.0)):
         with pytest.raises((NsrError, ValueError)):
             bad()
+
+
+@pytest.mark.parametrize("rows,width", [(37, 9001), (33, 12288), (21, 12289), (600, 5001), (300, 129), (1200, 1001), (530, 16384),
+                                        (700, 8192), (2100, 17), (257, 4), (1025, 7), (8200, 9), (300, 513), (70, 2049)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_group_and_access_boundaries(rows, width, dtype):
+    """widths around the sizes where rows go to larger groups of lanes, to the element-wise and to the long form; 16-bit rows at odd
+    addresses; row counts that leave the last tile of rows partly empty"""
+    from nsr_hip import ops
+    x, w, b, dy = _inputs(rows, width, dtype, F32, 11)
+    y, mean, rstd = ops.layer_norm_forward(x, w, b)
+    want, tol, m64, s64, (dm, ds) = _reference(x, w, b, 1e-5)
+    _close(y, want, tol, "y")
+    _close(mean, m64, dm, "mean")
+    _close(rstd, s64, ds, "rstd")
+    assert torch.equal(ops.layer_norm(x, w, b), y)
+    dx, dw, db = ops.layer_norm_backward(dy, x, w, mean, rstd)
+    (r, t), (rw, tw), (rb, tb) = _reference_backward(dy, x, w, mean, rstd)
+    _close(dx, r, t, "dx")
+    _close(dw, rw, tw + _store(rw, F32), "dweight")
+    _close(db, rb, tb + _store(rb, F32), "dbias")
+    for wants in ((True, False, False), (False, True, False), (False, False, True)):
+        part = ops.layer_norm_backward(dy, x, w, mean, rstd, *wants)
+        assert all((p is None) if not k else torch.equal(p, q) for k, p, q in zip(wants, part, (dx, dw, db)))
+
+
+@pytest.mark.parametrize("width", [64, 65, 257, 5001])
+def test_infinities_stay_in_their_row_and_columns(width):
+    """an infinite dy in the last row of a partly filled tile: the columns' sums are infinite there and exact elsewhere"""
+    from nsr_hip import ops
+    x, w, b, dy = _inputs(131, width, BF16, F32, 12)
+    _, mean, rstd = ops.layer_norm_forward(x, w, b)
+    clean = ops.layer_norm_backward(dy, x, w, mean, rstd)
+    dy[130, 3] = float("inf")
+    dx, dw, db = ops.layer_norm_backward(dy, x, w, mean, rstd)
+    assert torch.equal(dx[:130], clean[0][:130])
+    keep = torch.arange(width, device="cuda") != 3
+    assert torch.equal(dw[keep], clean[1][keep]) and torch.equal(db[keep], clean[2][keep])
+    assert float(db[3]) == float("inf") and torch.isinf(dw[3])
+
+
+def test_one_row_with_any_stride_through_the_c_entry():
+    """a single row has no stride: the C entry takes 0 for it (and no row past the end adds to the sums)"""
+    from nsr_hip import check, lib, ops, ptr, stream_ptr
+    x, w, b, dy = _inputs(1, 64, F32, F32, 13)
+    y, mean, rstd = ops.layer_norm_forward(x, w, b)
+    dx, dw, db = ops.layer_norm_backward(dy, x, w, mean, rstd)
+    y0, dx0, dw0, db0 = (torch.empty_like(t) for t in (y, dx, dw, db))
+    check(lib.nsr_layer_norm_forward(ptr(x), 0, ptr(w), ptr(b), ptr(y0), None, None, 1, 64, 0, 0, 1e-5, stream_ptr()))
+    check(lib.nsr_layer_norm_backward(ptr(dy), 0, ptr(x), 0, ptr(w), ptr(mean), ptr(rstd), ptr(dx0), ptr(dw0), ptr(db0), None, 1, 64,
+                                      0, 0, stream_ptr()))
+    assert all(torch.equal(p, q) for p, q in ((y, y0), (dx, dx0), (dw, dw0), (db, db0)))
