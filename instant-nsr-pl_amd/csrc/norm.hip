@@ -622,7 +622,8 @@ int narrow_group(uint32_t width, F f)
 
 // f(G, ITER) for rows of `width`: 1 vector a lane up to a wave, 8 columns a lane above it, the smallest G that covers the row.
 // (16 columns a lane of half as large groups: 74 instead of 69 us for both directions of 8192 x 4096 bf16.)  The widest group
-// takes more, as many as the registers hold: forward 16, backward (two sums and two inputs a column) 16 of 16 bits, 12 of fp32.
+// takes more, as many as the registers hold: forward 16, backward (two sums and two inputs a column) 16 of 16 bits, 12 of fp32;
+// wider rows, and in the backward pass 16-bit ones at odd addresses above 8192, go the long way.
 constexpr uint32_t FORWARD_MOST = 16384;
 constexpr uint32_t backward_most(uint32_t dtype) { return dtype == DT_F32 ? 12288 : 16384; }
 
@@ -664,6 +665,9 @@ uint32_t backward_groups(uint64_t rows, uint32_t width, uint32_t dtype)
             });
         });
     const uint64_t tiles = (rows + per - 1) / per, most = CUS;
+    // few rows: one workgroup does them all and needs no second launch (up to 4 tiles no slower alone, 12.9 instead of 16.8 us a
+    // call in a row of calls; 8 tiles are slower alone)
+    if (tiles <= 4) return 1;
     return (uint32_t)(tiles < most ? tiles : most);
 }
 
@@ -741,11 +745,15 @@ extern "C" int nsr_layer_norm_backward(const void *dy, uint64_t dy_stride, const
     hipStream_t st = (hipStream_t)stream;
     return ln_type(dtype, [&](auto t) {
         using T = decltype(t);
-        if (groups && width <= backward_most(dtype)) {
+        // (more than 8 columns a lane: in registers by buffer instructions only, the other form's addresses would not fit)
+        const bool wide = width > 8 * BWD_THREADS && access_of(width, dtype, x, x_stride, dx, width, dy, dy_stride, 1) != BUFFER;
+        if (groups && width <= backward_most(dtype) && !wide) {
             row_shape<T, backward_most(sizeof(T) == 4 ? DT_F32 : DT_F16)>(width, [&](auto g, auto iter) {
                 constexpr int G = decltype(g)::value, ITER = decltype(iter)::value;
                 const Access access = access_of(width, dtype, x, x_stride, dx, width, dy, dy_stride, BWD_THREADS / G);
-                auto kernel = access == BUFFER ? k_ln_backward<T, G, ITER, BUFFER> : k_ln_backward<T, G, ITER, GLOBAL>;
+                auto kernel = k_ln_backward<T, G, ITER, BUFFER>;
+                if constexpr (Vec16<T>::N * ITER <= 8)
+                    if (access == GLOBAL) kernel = k_ln_backward<T, G, ITER, GLOBAL>;
                 if constexpr (G == 1)
                     if (access == TINY) kernel = k_ln_backward<T, G, ITER, TINY>;
                 hipLaunchKernelGGL(kernel, dim3(groups), dim3(BWD_THREADS), 0, st,

@@ -846,24 +846,30 @@ def _rows(t, width):
 
 
 def _ln_check(x, weight, bias):
+    """refuses what the kernels do not take; the type of the affine parameters (the input's without any)"""
     if x.dtype not in DTYPE_CODES:
         raise NsrError(f"layer_norm: expected a float32/float16/bfloat16 tensor, got {x.dtype}")
     if not x.is_cuda:
         raise NsrError("nsr_hip ops need GPU tensors (there is no CPU path in the product library)")
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError(f"layer_norm: no last axis to normalise in shape {tuple(x.shape)}")
-    affine = None
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is None:
-            continue
-        if t.dim() != 1 or t.shape[0] != x.shape[-1]:
-            raise ValueError(f"layer_norm: {name} has shape {tuple(t.shape)}, expected ({x.shape[-1]},)")
-        if t.dtype != F32 and t.dtype != x.dtype or affine not in (None, t.dtype):
-            raise NsrError(f"layer_norm: weight and bias are both float32 or both {x.dtype}, got {t.dtype}")
-        if t.device != x.device:
-            raise NsrError(f"layer_norm: {name} is on {t.device}, the input on {x.device}")
-        affine = t.dtype
-    return x.dtype if affine is None else affine
+    if weight is not None:
+        _ln_check_affine("weight", weight, x)
+    if bias is not None:
+        _ln_check_affine("bias", bias, x)
+        if weight is not None and weight.dtype != bias.dtype:
+            raise NsrError(f"layer_norm: weight is {weight.dtype}, bias {bias.dtype}")
+        return bias.dtype
+    return x.dtype if weight is None else weight.dtype
+
+
+def _ln_check_affine(name, t, x):
+    if t.dim() != 1 or t.shape[0] != x.shape[-1]:
+        raise ValueError(f"layer_norm: {name} has shape {tuple(t.shape)}, expected ({x.shape[-1]},)")
+    if t.dtype != F32 and t.dtype != x.dtype:
+        raise NsrError(f"layer_norm: {name} is float32 or {x.dtype}, got {t.dtype}")
+    if t.device != x.device:
+        raise NsrError(f"layer_norm: {name} is on {t.device}, the input on {x.device}")
 
 
 def _addr(t):
