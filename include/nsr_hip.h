@@ -1083,6 +1083,12 @@ int nsr_grad_squares(const NsrAdamwTensor *tensors, uint32_t n_tensors, double *
 int nsr_adamw_begin(int32_t *step, float *hyper, double beta1, double beta2, const double *partials, uint32_t n_partials,
                     double max_norm, const float *grad_scale, const float *found_inf, void *stream);
 
+/* nsr_grad_squares over the tensors and nsr_adamw_begin with its sums, in one launch where there are few gradients.  partials:
+ * nsr_grad_squares_capacity doubles. */
+int nsr_adamw_begin_clipped(const NsrAdamwTensor *tensors, uint32_t n_tensors, double *partials, uint32_t capacity,
+                            int32_t *step, float *hyper, double beta1, double beta2, double max_norm, const float *grad_scale,
+                            const float *found_inf, void *stream);
+
 /* ------------------------------------------------------------------------------------------------
  * Layer norm over the last axis, for networks beside the fused 64-wide ones (the reference's VanillaMLP takes any torch layer:
  * models/network_utils.py:100-139).  Types as above; weight and bias (both may be NULL) are fp32 or of the input's type.

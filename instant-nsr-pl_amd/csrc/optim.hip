@@ -346,7 +346,7 @@ __device__ __forceinline__ double chunk_squares(const void *grad, uint64_t n, ui
     Vec<T, N> v[PASSES];
 #pragma unroll
     for (int it = 0; it < PASSES; ++it) {
-        const uint32_t i = (it * OPT_THREADS + threadIdx.x) * N;
+        const uint32_t i = (it * OPT_THREADS + threadIdx.x % OPT_THREADS) * N;
         if (i + N <= left) {
             v[it] = get<Vec<T, N>>(g + i);
         } else {
@@ -368,11 +368,11 @@ __device__ __forceinline__ double wave_sum64(double v)
     return v;
 }
 
-__global__ void __launch_bounds__(OPT_THREADS)
-k_grad_squares(const NormLaunch a, double *__restrict__ partials)
+// sums of squares of every `stride`th chunk from `chunk` on, by 256 threads
+__device__ __forceinline__ double squares_of_chunks(const NormLaunch &a, uint32_t chunk, uint32_t stride)
 {
     double acc = 0.0;
-    for (uint32_t chunk = blockIdx.x; chunk < a.n_chunks; chunk += gridDim.x) {
+    for (; chunk < a.n_chunks; chunk += stride) {
         const uint32_t which = tensor_of(a, chunk);
         const NormTensor &t = a.t[which];
         const uint64_t n = t.size & ((1ull << SIZE_BITS) - 1), base = (uint64_t)(chunk - a.first[which]) * NORM_CHUNK;
@@ -381,49 +381,77 @@ k_grad_squares(const NormLaunch a, double *__restrict__ partials)
         else if (dt == DT_F16) acc += chunk_squares<DT_F16>(t.g, n, base);
         else acc += chunk_squares<DT_BF16>(t.g, n, base);
     }
+    return acc;
+}
+
+__global__ void __launch_bounds__(OPT_THREADS)
+k_grad_squares(const NormLaunch a, double *__restrict__ partials)
+{
+    const double acc = wave_sum64(squares_of_chunks(a, blockIdx.x, gridDim.x));
     __shared__ double part[OPT_THREADS / 64];
-    acc = wave_sum64(acc);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = acc;
     __syncthreads();
     if (threadIdx.x == 0) partials[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-// one workgroup: the partial sums in a fixed order, then the step's scalars.  Two threads have worked out b^t = exp(t ln b) in 64
-// bits meanwhile (its error, t |ln b| 2^-53 of it, is far under fp32's; pow took twice as long as the whole kernel does now).
+// one workgroup: each thread's share of the sum of squares in a fixed order, then the step's scalars.  Two threads have worked
+// out b^t = exp(t ln b) in 64 bits meanwhile (its error, t |ln b| 2^-53 of it, is far under fp32's; pow took twice as long as
+// the whole kernel does now).
 constexpr int BEGIN_THREADS = 1024;
-__global__ void __launch_bounds__(BEGIN_THREADS)
-k_adamw_begin(int32_t *__restrict__ step, float *__restrict__ hyper, double ln_b1, double ln_b2,
-              const double *__restrict__ partials, uint32_t n_partials, double max_norm, const float *__restrict__ grad_scale,
-              const float *__restrict__ found_inf)
+struct Begin {
+    int32_t *step;
+    float *hyper;
+    double ln_b1, ln_b2, max_norm;
+    const float *grad_scale, *found_inf;
+};
+__device__ __forceinline__ void begin_step(const Begin &b, double acc, bool clip)
 {
     __shared__ double part[BEGIN_THREADS / 64], power[2];
-    const int32_t taken = *step;
-    double acc = 0.0;
-    for (uint32_t i = threadIdx.x; i < n_partials; i += BEGIN_THREADS) acc += partials[i];
-    if (threadIdx.x == 64 || threadIdx.x == 128) power[threadIdx.x / 128] = exp((taken + 1.0) * (threadIdx.x == 64 ? ln_b1 : ln_b2));
+    const int32_t taken = *b.step;
+    if (threadIdx.x == 64 || threadIdx.x == 128)
+        power[threadIdx.x / 128] = exp((taken + 1.0) * (threadIdx.x == 64 ? b.ln_b1 : b.ln_b2));
     acc = wave_sum64(acc);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = acc;
     __syncthreads();
     if (threadIdx.x != 0) return;
-    const double unscale = grad_scale ? 1.0 / (double)*grad_scale : 1.0;
+    const double unscale = b.grad_scale ? 1.0 / (double)*b.grad_scale : 1.0;
     double factor = unscale;
-    bool skip = found_inf && *found_inf != 0.f;
-    if (partials) {
+    bool skip = b.found_inf && *b.found_inf != 0.f;
+    if (clip) {
         double sum = part[0];
         for (int k = 1; k < BEGIN_THREADS / 64; ++k) sum += part[k];
         const double norm = sqrt(sum) * unscale;
-        const double ratio = max_norm / (norm + 1e-6);  // torch.nn.utils.clip_grad_norm_
+        const double ratio = b.max_norm / (norm + 1e-6);  // torch.nn.utils.clip_grad_norm_
         factor *= ratio < 1.0 ? ratio : 1.0;
         skip = skip || !(norm <= 1.7976931348623157e308);
-        hyper[5] = (float)norm;
+        b.hyper[5] = (float)norm;
     }
-    if (!skip) *step = taken + 1;
-    hyper[0] = (float)factor;
-    hyper[1] = (float)(1.0 / (1.0 - power[0]));
-    hyper[2] = (float)(1.0 / sqrt(1.0 - power[1]));
-    hyper[3] = __int_as_float(skip ? 1 : 0);
-    hyper[4] = __int_as_float(taken + 1);  // (read only where the step is taken)
+    if (!skip) *b.step = taken + 1;
+    b.hyper[0] = (float)factor;
+    b.hyper[1] = (float)(1.0 / (1.0 - power[0]));
+    b.hyper[2] = (float)(1.0 / sqrt(1.0 - power[1]));
+    b.hyper[3] = __int_as_float(skip ? 1 : 0);
+    b.hyper[4] = __int_as_float(taken + 1);  // (read only where the step is taken)
 }
+
+__global__ void __launch_bounds__(BEGIN_THREADS)
+k_adamw_begin(const Begin b, const double *__restrict__ partials, uint32_t n_partials)
+{
+    double acc = 0.0;
+    for (uint32_t i = threadIdx.x; i < n_partials; i += BEGIN_THREADS) acc += partials[i];
+    begin_step(b, acc, partials != nullptr);
+}
+
+// few gradients: the workgroup sums their squares itself, four chunks at a time
+__global__ void __launch_bounds__(BEGIN_THREADS)
+k_adamw_begin_few(const Begin b, const NormLaunch a)
+{
+    constexpr uint32_t AT_ONCE = BEGIN_THREADS / OPT_THREADS;
+    begin_step(b, squares_of_chunks(a, (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x / OPT_THREADS), AT_ONCE), true);
+}
+static_assert(sizeof(NormLaunch) + sizeof(Begin) <= 3840, "kernel arguments stay under 4 KB");
+// (up to 131072 elements; a clipped step of that size: 18.2 us a call, 20.6 us with the sums in a launch of their own)
+constexpr uint32_t FEW_CHUNKS = 32;
 
 // ---- host ----------------------------------------------------------------------------------------------------------------
 // 2^23 chunks of 256 threads are 2^31 threads: a grid stays under the launch limit of 2^32 with the next tensor's chunks too.
@@ -485,6 +513,12 @@ int each_launch(const NsrAdamwTensor *tensors, uint32_t n_tensors, uint32_t chun
     return a.n_tensors ? go(a) : NSR_OK;
 }
 
+void fill_norm(NormTensor &t, const NsrAdamwTensor &x, uint64_t at, uint64_t n)
+{
+    t.g = (const char *)x.grad + at * dtype_size(x.dtype);
+    t.size = n | (uint64_t)x.dtype << SIZE_BITS;
+}
+
 }  // namespace
 
 extern "C" int nsr_adamw_tensors(const NsrAdamwTensor *tensors, uint32_t n_tensors, double beta1, double beta2, double eps,
@@ -543,11 +577,7 @@ extern "C" int nsr_grad_squares(const NsrAdamwTensor *tensors, uint32_t n_tensor
     *n_partials = 0;
     const int rc = check_grads("nsr_grad_squares", tensors, n_tensors);
     if (rc != NSR_OK) return rc;
-    auto fill = [](NormTensor &t, const NsrAdamwTensor &x, uint64_t at, uint64_t n) {
-        t.g = (const char *)x.grad + at * dtype_size(x.dtype);
-        t.size = n | (uint64_t)x.dtype << SIZE_BITS;
-    };
-    return each_launch<NormTensor, 128>(tensors, n_tensors, NORM_CHUNK, fill, [&](const NormLaunch &a) {
+    return each_launch<NormTensor, 128>(tensors, n_tensors, NORM_CHUNK, fill_norm, [&](const NormLaunch &a) {
         const uint32_t grid = a.n_chunks < NORM_MAX_GRID ? a.n_chunks : NORM_MAX_GRID;
         NSR_REQUIRE(capacity - *n_partials >= grid, "nsr_grad_squares: room for %u partial sums is too little", capacity);
         hipLaunchKernelGGL(k_grad_squares, dim3(grid), dim3(OPT_THREADS), 0, (hipStream_t)stream, a, partials + *n_partials);
@@ -564,8 +594,32 @@ extern "C" int nsr_adamw_begin(int32_t *step, float *hyper, double beta1, double
     NSR_REQUIRE(step && hyper, "nsr_adamw_begin: NULL pointer");
     NSR_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "nsr_adamw_begin: betas in [0, 1)");
     NSR_REQUIRE(!partials || max_norm > 0.0, "nsr_adamw_begin: max_norm > 0");
-    hipLaunchKernelGGL(k_adamw_begin, dim3(1), dim3(BEGIN_THREADS), 0, (hipStream_t)stream, step, hyper, log(beta1), log(beta2),
-                       partials, partials ? n_partials : 0, max_norm, grad_scale, found_inf);
+    const Begin b{step, hyper, log(beta1), log(beta2), max_norm, grad_scale, found_inf};
+    hipLaunchKernelGGL(k_adamw_begin, dim3(1), dim3(BEGIN_THREADS), 0, (hipStream_t)stream, b, partials, partials ? n_partials : 0);
     NSR_CHECK_LAUNCH("nsr_adamw_begin");
     return NSR_OK;
+}
+
+extern "C" int nsr_adamw_begin_clipped(const NsrAdamwTensor *tensors, uint32_t n_tensors, double *partials, uint32_t capacity,
+                                       int32_t *step, float *hyper, double beta1, double beta2, double max_norm,
+                                       const float *grad_scale, const float *found_inf, void *stream)
+{
+    NSR_REQUIRE(step && hyper && partials, "nsr_adamw_begin_clipped: NULL pointer");
+    NSR_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "nsr_adamw_begin_clipped: betas in [0, 1)");
+    NSR_REQUIRE(max_norm > 0.0, "nsr_adamw_begin_clipped: max_norm > 0");
+    int rc = check_grads("nsr_adamw_begin_clipped", tensors, n_tensors);
+    if (rc != NSR_OK) return rc;
+    uint64_t chunks = 0, live = 0;
+    for (uint32_t i = 0; i < n_tensors; ++i) { chunks += nsr_div_up(tensors[i].n, NORM_CHUNK); live += tensors[i].n != 0; }
+    if (chunks == 0 || chunks > FEW_CHUNKS || live > 128) {
+        uint32_t n = 0;
+        rc = nsr_grad_squares(tensors, n_tensors, partials, capacity, &n, stream);
+        return rc != NSR_OK ? rc : nsr_adamw_begin(step, hyper, beta1, beta2, partials, n, max_norm, grad_scale, found_inf, stream);
+    }
+    const Begin b{step, hyper, log(beta1), log(beta2), max_norm, grad_scale, found_inf};
+    return each_launch<NormTensor, 128>(tensors, n_tensors, NORM_CHUNK, fill_norm, [&](const NormLaunch &a) {
+        hipLaunchKernelGGL(k_adamw_begin_few, dim3(1), dim3(BEGIN_THREADS), 0, (hipStream_t)stream, b, a);
+        NSR_CHECK_LAUNCH("nsr_adamw_begin_clipped");
+        return NSR_OK;
+    });
 }

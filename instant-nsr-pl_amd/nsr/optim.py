@@ -1,6 +1,5 @@
 """AdamW over any number of tensors for a user's own training system (the reference's ``parse_optimizer`` builds
 ``torch.optim.AdamW``: systems/utils.py:314-325; the trainers of this package own their optimizers and do not need it)."""
-import ctypes
 import math
 
 import numpy as np
@@ -293,21 +292,20 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def _begin(self, desc, n, b1, b2, scale, found, stream):
-        count, partials, clip = 0, None, 0.0
-        if self.max_grad_norm is not None:
-            if self._partials is None:
-                room = lib.nsr_grad_squares_capacity(self._desc, len(self._ps))
-                self._partials = torch.empty(room, dtype=torch.float64, device=self.device)
-            got = ctypes.c_uint32()
-            check(lib.nsr_grad_squares(desc, n, self._partials.data_ptr(), self._partials.numel(), ctypes.byref(got), stream),
-                  "nsr_grad_squares")
-            count, partials, clip = got.value, self._partials.data_ptr(), self.max_grad_norm
         for t in (scale, found):
             if t is not None and (t.dtype != F32 or t.device != self.device or t.numel() != 1):
                 raise NsrError("AdamW: grad_scale and found_inf are one float32 element on the parameters' device")
-        check(lib.nsr_adamw_begin(ptr(self._step_dev), ptr(self._hyper), b1, b2, partials, count, clip,
-                                  None if scale is None else scale.data_ptr(), None if found is None else found.data_ptr(),
-                                  stream), "nsr_adamw_begin")
+        step, hyper = self._step_dev.data_ptr(), self._hyper.data_ptr()
+        scale = None if scale is None else scale.data_ptr()
+        found = None if found is None else found.data_ptr()
+        if self.max_grad_norm is None:
+            check(lib.nsr_adamw_begin(step, hyper, b1, b2, None, 0, 0.0, scale, found, stream), "nsr_adamw_begin")
+            return
+        if self._partials is None:
+            room = lib.nsr_grad_squares_capacity(self._desc, len(self._ps))
+            self._partials = torch.empty(room, dtype=torch.float64, device=self.device)
+        check(lib.nsr_adamw_begin_clipped(desc, n, self._partials.data_ptr(), self._partials.numel(), step, hyper, b1, b2,
+                                          self.max_grad_norm, scale, found, stream), "nsr_adamw_begin_clipped")
 
     # ---- checkpoints ---------------------------------------------------------------------------------------------------------
     def state_dict(self):

@@ -265,6 +265,7 @@ SIGNATURES = {
     "nsr_adamw_tensors": [_P, _U, _D, _D, _D, ctypes.c_int32, _P, _D, _U, _P],
     "nsr_grad_squares_capacity": [_P, _U],
     "nsr_grad_squares": [_P, _U, _P, _U, ctypes.POINTER(ctypes.c_uint32), _P],
+    "nsr_adamw_begin_clipped": [_P, _U, _P, _U, _P, _P, _D, _D, _D, _P, _P, _P],
     "nsr_adamw_begin": [_P, _P, _D, _D, _P, _U, _D, _P, _P, _P],
     "nsr_layer_norm_forward": [_P, _U64, _P, _P, _P, _P, _P, _U64, _U, _U, _U, _F, _P],
     "nsr_layer_norm_backward_workspace_floats": [_U64, _U, _U],

@@ -110,3 +110,16 @@ def test_descriptor_layout(tmp_path):
     subprocess.check_call(["gcc", "-I", os.path.join(ROOT, "include"), "-o", str(exe), str(src)])
     got = [int(v) for v in subprocess.check_output([str(exe)], text=True).split()]
     assert got == [ctypes.sizeof(cls)] + [getattr(cls, f[0]).offset for f in cls._fields_]
+
+
+def test_begin_clipped_refuses():
+    import nsr_hip
+    call = nsr_hip.lib.nsr_adamw_begin_clipped
+    t = _tensor()
+    good = (t, 1, 4096, 10000, 4096, 4096, 0.9, 0.99, 1.0, None, None, None)
+    for at, bad in ((0, None), (2, None), (4, None), (5, None), (6, 1.0), (7, -0.1), (8, 0.0), (8, float("nan"))):
+        args = list(good)
+        args[at] = bad
+        assert call(*args) < 0, at
+    assert call(_tensor(grad=None), *good[1:]) < 0 and call(_tensor(dtype=7), *good[1:]) < 0
+    assert call(_tensor(n=1 << 30), 1, 4096, 10, *good[4:]) < 0  # too little room for the sums, refused before a launch
