@@ -227,7 +227,8 @@ __device__ __forceinline__ void load_affine(const void *p, bool fp32, uint32_t c
 }
 
 // ---- forward ---------------------------------------------------------------------------------------------------------------
-// A lane's weight and bias stay in registers.  Groups of more than a wave load the next row while they work on one; smaller ones
+// Two sums over the row's registers (mean, then squares about it), one fma an element with weight and bias, which stay in
+// registers.  Bound by HBM: 2097152 x 64 fp16 in 94 us (5.7 TB/s), 8192 x 4096 bf16 in 25 us (5.3 TB/s).  Groups of more than a wave load the next row while they work on one; smaller ones
 // have enough waves without (2097152 x 64 fp16: 94 us without, 101 us with).
 template <class T, int G, int ITER, Access A>
 __global__ void __launch_bounds__(G > 256 ? G : 256)
@@ -353,7 +354,10 @@ __device__ __forceinline__ void store_sum(int which, uint32_t col, float v, uint
     }
 }
 
-// The next row of each group is under way as soon as this one is in fp32 registers.  (Two rows ahead: 43.8 instead of 41.1 us
+// Bound by HBM: 262144 x 64 fp32 in 34 us (6.0 TB/s, a part of it cached), 131072 x 256 bf16 in 35 us (5.8 TB/s), 8192 x 4096
+// bf16 in 38 us (5.4 TB/s with the partial sums); the launch that adds those takes 4 to 5 us.  1024 threads a workgroup, one
+// workgroup a CU: halves or quarters of that with as many more workgroups only made more partial sums (8192 x 4096 bf16 as a
+// whole 69.7 and 76.5 us).  The next row of each group is under way as soon as this one is in fp32 registers.  (Two rows ahead: 43.8 instead of 41.1 us
 // for 262144 x 64 fp32, 44.6 instead of 41.8 us for 131072 x 256 bf16.)
 template <class T, int G, int ITER, Access A>
 __global__ void __launch_bounds__(BWD_THREADS)
