@@ -67,6 +67,9 @@ class AdamW(torch.optim.Optimizer):
             self._learning_rate(g)
         if self.capturable or self.max_grad_norm is not None:
             self._device_step()
+        if self.max_grad_norm is not None:
+            room = lib.nsr_grad_squares_capacity(self._desc, len(self._ps))
+            self._partials = torch.empty(room, dtype=torch.float64, device=self.device)
         self._built = True
 
     # ---- construction --------------------------------------------------------------------------------------------------------
@@ -93,6 +96,7 @@ class AdamW(torch.optim.Optimizer):
         self._group_of = [i for _, i in items]
         self._all_contiguous = all(p.is_contiguous() for p in self._ps)
         self._addresses = [p.data_ptr() for p in self._ps]
+        self._nbytes = [p.nbytes for p in self._ps]
         self._bits = [8 if self.state_bits == 8 and p.numel() >= self.min_8bit_size else 32 for p in self._ps]
         self._at, total = [], {8: 0, 32: 0}
         for p, bits in zip(self._ps, self._bits):
@@ -224,21 +228,29 @@ class AdamW(torch.optim.Optimizer):
             for i, (p, g) in enumerate(zip(ps, grads)):
                 if g is None:
                     continue
-                if g.is_sparse:
-                    raise NsrError("AdamW: sparse gradients are not supported")
+                if g.layout is not torch.strided:
+                    raise NsrError(f"AdamW: a gradient of layout {g.layout} is not supported")
                 if g.stride() != p.stride() and p.numel():  # in the parameter's order of elements
                     grads[i] = torch.empty_strided(p.shape, p.stride(), dtype=p.dtype, device=p.device)
                     with torch.no_grad():
                         grads[i].copy_(g)
             keep = grads
             live = [i for i, g in enumerate(grads) if g is not None]
+            self._check_sizes([grads[i].nbytes for i in live], [self._nbytes[i] for i in live])
             if len(live) < len(ps):
                 for i in live:
                     f["grad"][i] = grads[i].data_ptr()
                 some = f[live]  # (a copy)
                 return some.ctypes.data, len(live), [ps[i] for i in live], (keep, some)
+        self._check_sizes([g.nbytes for g in grads], self._nbytes)
         f["grad"] = [g.data_ptr() for g in grads]
         return self._desc, len(ps), ps, keep
+
+    @staticmethod
+    def _check_sizes(got, want):
+        # torch sees to it for ``p.grad = g``, but not for ``p.grad.data = g`` or a ``grad_dtype`` of its own
+        if got != want:
+            raise NsrError("AdamW: a gradient has another size or type than its parameter")
 
     def _check_moved(self):
         """parameters whose memory was replaced (``p.data = ...``) still have the layout that the moments were made for"""
@@ -301,9 +313,6 @@ class AdamW(torch.optim.Optimizer):
         if self.max_grad_norm is None:
             check(lib.nsr_adamw_begin(step, hyper, b1, b2, None, 0, 0.0, scale, found, stream), "nsr_adamw_begin")
             return
-        if self._partials is None:
-            room = lib.nsr_grad_squares_capacity(self._desc, len(self._ps))
-            self._partials = torch.empty(room, dtype=torch.float64, device=self.device)
         check(lib.nsr_adamw_begin_clipped(desc, n, self._partials.data_ptr(), self._partials.numel(), step, hyper, b1, b2,
                                           self.max_grad_norm, scale, found, stream), "nsr_adamw_begin_clipped")
 
@@ -318,6 +327,8 @@ class AdamW(torch.optim.Optimizer):
         """state of an optimizer with the same tensors and the same ``state_bits`` for each of them (the moments keep their own
         types, unlike in torch, which casts them to the parameter's)"""
         saved, steps = state_dict["state"], set()
+        if any(g.get("amsgrad") or g.get("maximize") for g in state_dict["param_groups"]):
+            raise NotImplementedError("AdamW: neither amsgrad nor maximize")
         for i, p in enumerate(self._ps):
             if i not in saved or not p.numel():
                 continue
@@ -326,10 +337,17 @@ class AdamW(torch.optim.Optimizer):
                 if v is None or v.dtype != t.dtype or v.shape != t.shape:
                     raise ValueError(f"AdamW.load_state_dict: tensor {i} needs {k} {tuple(t.shape)} {t.dtype}, the state has "
                                      f"{None if v is None else (tuple(v.shape), v.dtype)}")
+            if "step" not in saved[i]:
+                raise ValueError(f"AdamW.load_state_dict: the state of tensor {i} has no step count")
             steps.add(float(saved[i]["step"]))
         if len(steps) > 1:
             raise ValueError(f"AdamW.load_state_dict: the tensors' step counts differ: {sorted(steps)}")
+        rates = [g["lr"] for g in self.param_groups]
         super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
+        for g, lr in zip(self.param_groups, rates):
+            if isinstance(lr, torch.Tensor):  # (a captured step reads this tensor: it keeps its place)
+                lr.fill_(float(g["lr"]))
+                g["lr"] = lr
         self._bind_state()
         for i, p in enumerate(self._ps):
             for k, t in self.state.get(p, {}).items():

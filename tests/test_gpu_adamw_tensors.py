@@ -537,3 +537,74 @@ def test_refusals_on_the_gpu():
     p.data = torch.zeros(7, device="cuda")
     with pytest.raises(NsrError):
         opt.step()
+
+
+def test_replaced_gradients_are_refused_and_copies_too():
+    import copy
+    import nsr.optim
+    from nsr_hip import NsrError
+    ps, opt, grads = _make([600, 33], F32, lr=0.01)
+    for p, g in zip(ps, grads()):
+        p.grad = g
+    ps[0].grad.data = torch.zeros(599, device="cuda")  # (torch checks ``p.grad = g``, not this)
+    before = [p.detach().clone() for p in ps]
+    with pytest.raises(NsrError):
+        opt.step()
+    ps[1].grad = None
+    with pytest.raises(NsrError):
+        opt.step()
+    assert all(torch.equal(p, q) for p, q in zip(ps, before)) and opt.taken_steps() == 0
+    ps[1].grad, ps[0].grad = torch.sparse_coo_tensor(torch.tensor([[1]]), torch.ones(1), (33,)).cuda(), None
+    with pytest.raises((NsrError, RuntimeError)):
+        opt.step()
+    with pytest.raises(NotImplementedError):
+        copy.deepcopy(opt)
+    q = torch.nn.Parameter(torch.zeros(5, device="cuda"))
+    theirs = torch.optim.AdamW([q], amsgrad=True)
+    with pytest.raises(NotImplementedError):
+        nsr.optim.AdamW([torch.nn.Parameter(torch.zeros(5, device="cuda"))]).load_state_dict(theirs.state_dict())
+
+
+def test_closure_hooks_and_a_rate_that_keeps_its_place():
+    import nsr.optim
+    p = torch.nn.Parameter(torch.ones(300, device="cuda"))
+    lr = torch.tensor(0.5, device="cuda")
+    opt = nsr.optim.AdamW([p], lr=lr, weight_decay=0.0, capturable=True)
+    seen = []
+    opt.register_step_pre_hook(lambda *a: seen.append("before"))
+    opt.register_step_post_hook(lambda *a: seen.append("after"))
+
+    def closure():
+        opt.zero_grad()
+        loss = (p * 2).sum()
+        loss.backward()
+        return loss
+
+    assert float(opt.step(closure)) == 600.0 and seen == ["before", "after"]
+    assert torch.allclose(p, torch.full_like(p, 0.5), atol=1e-6)
+    sd = opt.state_dict()
+    sd["param_groups"][0]["lr"] = torch.tensor(0.25)
+    opt.load_state_dict(sd)
+    assert opt.param_groups[0]["lr"] is lr and float(lr) == 0.25 and opt.taken_steps() == 1
+
+
+def test_pieces_of_one_tensor():
+    """2^33 + 4099 elements are two pieces of one launch each: those around the cut and the last ones move like the others"""
+    import nsr.optim
+    n = (1 << 33) + 4099
+    p = torch.nn.Parameter(torch.zeros(n, dtype=BF16, device="cuda"))
+    p.grad = torch.zeros(n, dtype=BF16, device="cuda")
+    opt = nsr.optim.AdamW([p], lr=0.5, weight_decay=0.0, state_bits=8, rounding_seed=9)
+    cut = 1 << 33
+    where = torch.cat([torch.arange(3), torch.arange(cut - 300, cut + 300), torch.arange(n - 5, n)]).cuda()
+    g = torch.linspace(0.5, 2.0, where.numel(), device="cuda").to(BF16)
+    p.grad[where] = g
+    opt.step()
+    assert torch.equal(p[where], torch.full_like(g, -0.5))
+    assert sum(int(torch.count_nonzero(part)) for part in p.detach().split(1 << 31)) == where.numel()
+    s = opt.state[p]
+    m = torch.zeros(1024, dtype=torch.float64, device="cuda")
+    m[212:812] = 0.1 * g[3:603].double()  # elements cut - 512 .. cut + 511
+    e = cut - 512 + torch.arange(1024, device="cuda")
+    b0 = (cut - 512) // 256
+    _codes_match(s["exp_avg"][cut - 512:cut + 512], s["scales"][0, b0:b0 + 4], m, 6 * U * m.abs(), _bits(9, 1, e) >> 16, 0.0)
