@@ -9,6 +9,7 @@ from nsr_hip import NsrAdamwTensor, NsrError, check, device_guard, lib, ptr, str
 from nsr_hip.ops import DTYPE_CODES, timed
 
 F32, F8 = torch.float32, torch.float8_e4m3fn
+_DESCRIPTOR = np.dtype(NsrAdamwTensor)
 BLOCK = 256  # elements under one scale of the 8-bit moments (csrc/optim.hip); every tensor's moments start at a multiple of it
 
 
@@ -98,46 +99,50 @@ class AdamW(torch.optim.Optimizer):
         self._addresses = [p.data_ptr() for p in self._ps]
         self._nbytes = [p.nbytes for p in self._ps]
         self._bits = [8 if self.state_bits == 8 and p.numel() >= self.min_8bit_size else 32 for p in self._ps]
-        self._at, total = [], {8: 0, 32: 0}
-        for p, bits in zip(self._ps, self._bits):
-            self._at.append(total[bits])
-            total[bits] += -(-p.numel() // BLOCK) * BLOCK
-        new = lambda n, dtype: torch.zeros(n, dtype=torch.uint8 if dtype is F8 else dtype, device=self.device).view(dtype)  # noqa: E731
+        n = np.array([p.numel() for p in self._ps], dtype=np.int64)
+        eight = np.array([b == 8 for b in self._bits])
+        room = -(-n // BLOCK) * BLOCK
         # flat moments: tensor i has [at, at + numel) of the set of its width, zeros behind it up to the next multiple of BLOCK
-        self.flat32 = {k: new(total[32], F32) for k in ("exp_avg", "exp_avg_sq")} if total[32] else {}
+        at = np.where(eight, np.cumsum(room * eight) - room, np.cumsum(room * ~eight) - room)
+        self._at, total8, total32 = at.tolist(), int((room * eight).sum()), int((room * ~eight).sum())
+        zeros = lambda n, dtype: torch.zeros(n, dtype=torch.uint8 if dtype is F8 else dtype, device=self.device).view(dtype)  # noqa: E731
+        self.flat32 = {k: zeros(total32, F32) for k in ("exp_avg", "exp_avg_sq")} if total32 else {}
         self.flat8 = {}
-        if total[8]:
-            self.flat8 = {k: new(total[8], F8) for k in ("exp_avg", "exp_avg_rms")}
-            self.flat8["scales"] = torch.zeros(2, total[8] // BLOCK, dtype=F32, device=self.device)
-        n = len(self._ps)
-        self._desc = (NsrAdamwTensor * n)()
-        self._fields = np.frombuffer(self._desc, dtype=np.dtype(NsrAdamwTensor))
-        f = self._fields
-        f["n"] = [p.numel() for p in self._ps]
+        if total8:
+            self.flat8 = {k: zeros(total8, F8) for k in ("exp_avg", "exp_avg_rms")}
+            self.flat8["scales"] = torch.zeros(2, total8 // BLOCK, dtype=F32, device=self.device)
+        self._desc = (NsrAdamwTensor * len(self._ps))()
+        f = self._fields = np.frombuffer(self._desc, dtype=_DESCRIPTOR)
+        f["n"], f["index0"], f["state_bits"] = n, at, self._bits
         f["params"] = self._addresses
         f["dtype"] = [DTYPE_CODES[p.dtype] for p in self._ps]
-        f["state_bits"] = self._bits
-        f["index0"] = self._at
-        for i, (at, bits) in enumerate(zip(self._at, self._bits)):
-            if bits == 8:
-                d = self._desc[i]
-                d.exp_avg, d.exp_avg_sq = self.flat8["exp_avg"].data_ptr() + at, self.flat8["exp_avg_rms"].data_ptr() + at
-                d.scales_m = self.flat8["scales"].data_ptr() + 4 * (at // BLOCK)
-                d.scales_r = d.scales_m + 4 * self.flat8["scales"].shape[1]
-            elif f["n"][i]:
-                d = self._desc[i]
-                d.exp_avg, d.exp_avg_sq = (self.flat32[k].data_ptr() + 4 * at for k in ("exp_avg", "exp_avg_sq"))
+        for flat, size, which in ((self.flat32, 4, ~eight & (n > 0)), (self.flat8, 1, eight)):
+            if flat and which.any():
+                first, second = list(flat)[:2]
+                f["exp_avg"][which] = flat[first].data_ptr() + size * at[which]
+                f["exp_avg_sq"][which] = flat[second].data_ptr() + size * at[which]
+        if total8:
+            f["scales_m"][eight] = self.flat8["scales"].data_ptr() + 4 * (at[eight] // BLOCK)
+            f["scales_r"][eight] = f["scales_m"][eight] + 4 * (total8 // BLOCK)
         self._bind_state()
 
     def _bind_state(self):
-        for p, at, bits in zip(self._ps, self._at, self._bits):
-            flat, n = self.flat8 if bits == 8 else self.flat32, p.numel()
-            if not n:
+        """``self.state`` as views of the flat moments, in the parameters' shapes and orders of elements"""
+        for flat, width in ((self.flat32, 32), (self.flat8, 8)):
+            ps = [p for p, bits in zip(self._ps, self._bits) if bits == width and p.numel()]
+            if not ps:
                 continue
-            s = {k: t[at:at + n].as_strided(p.shape, p.stride()) for k, t in flat.items() if k != "scales"}
-            if bits == 8:
-                s["scales"] = flat["scales"][:, at // BLOCK:-(-(at + n) // BLOCK)]
-            self.state[p] = s
+            room = [-(-p.numel() // BLOCK) * BLOCK for p in ps]
+            views = {k: t.split(room) if k != "scales" else t.split([r // BLOCK for r in room], dim=1) for k, t in flat.items()}
+            for i, p in enumerate(ps):
+                s = self.state[p] = {}
+                for k, v in views.items():
+                    if k == "scales":
+                        s[k] = v[i]
+                    elif p.dim() == 1 and p.numel() == room[i]:
+                        s[k] = v[i]
+                    else:
+                        s[k] = v[i].as_strided(p.shape, p.stride())
 
     def _image_modules(self, modules):
         place = {id(p): i for i, p in enumerate(self._ps)}
