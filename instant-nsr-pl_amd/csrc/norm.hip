@@ -356,9 +356,9 @@ __device__ __forceinline__ void store_sum(int which, uint32_t col, float v, uint
 
 // Bound by HBM: 262144 x 64 fp32 in 34 us (6.0 TB/s, a part of it cached), 131072 x 256 bf16 in 35 us (5.8 TB/s), 8192 x 4096
 // bf16 in 38 us (5.4 TB/s with the partial sums); the launch that adds those takes 4 to 5 us.  1024 threads a workgroup, one
-// workgroup a CU: halves or quarters of that with as many more workgroups only made more partial sums (8192 x 4096 bf16 as a
-// whole 69.7 and 76.5 us).  The next row of each group is under way as soon as this one is in fp32 registers.  (Two rows ahead: 43.8 instead of 41.1 us
-// for 262144 x 64 fp32, 44.6 instead of 41.8 us for 131072 x 256 bf16.)
+// workgroup a CU: halves or quarters of that with as many more workgroups only made more partial sums (both directions of
+// 8192 x 4096 bf16: 69.7 and 76.5 us).  The next row of each group is under way as soon as this one is in fp32 registers.  (Two
+// rows ahead: 43.8 instead of 41.1 us for 262144 x 64 fp32, 44.6 instead of 41.8 us for 131072 x 256 bf16.)
 template <class T, int G, int ITER, Access A>
 __global__ void __launch_bounds__(BWD_THREADS)
 k_ln_backward(const T *__restrict__ dy, uint64_t dys, const T *__restrict__ x, uint64_t xs, const void *__restrict__ w,

@@ -39,6 +39,9 @@ class AdamW(torch.optim.Optimizer):
     ``modules``: ``tinycudann`` modules whose ``params`` are among the parameters: the fp16 image that their kernels read is
     written in the same pass (otherwise they cast ``params`` again in every forward pass).
 
+    ``flat32`` / ``flat8``: the moments of all tensors as one buffer each (``state`` holds views of them); ``set_step`` and
+    ``taken_steps``: the step count.
+
     Parameters are float32, float16 or bfloat16 (arithmetic and 32-bit moments in float32), dense and on one GPU; ``betas`` and
     ``eps`` are the same for all groups, ``lr`` and ``weight_decay`` are the group's.  Tensors whose ``grad`` is None are left
     as they are; the step count is one for all tensors.  An element whose gradient is not finite keeps its value and moments.
