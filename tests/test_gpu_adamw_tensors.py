@@ -608,3 +608,23 @@ def test_pieces_of_one_tensor():
     e = cut - 512 + torch.arange(1024, device="cuda")
     b0 = (cut - 512) // 256
     _codes_match(s["exp_avg"][cut - 512:cut + 512], s["scales"][0, b0:b0 + 4], m, 6 * U * m.abs(), _bits(9, 1, e) >> 16, 0.0)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_more_tensors_than_a_launch_takes(bits):
+    """300 tensors: several launches of the update (64, 36) and of the norm (128), against the formula"""
+    lr, betas, eps, wd = 0.01, (0.9, 0.99), 1e-15, 0.1
+    sizes = [37 + k for k in range(299)] + [9000]
+    ps, opt, grads = _make(sizes, F32, lr=lr, betas=betas, eps=eps, weight_decay=wd, state_bits=bits, min_8bit_size=0,
+                           max_grad_norm=0.5)
+    for t in (1, 2):
+        gs = grads()
+        for p, g in zip(ps, gs):
+            p.grad = g
+        before = [(p.detach().clone(), *_moments(opt, p)) for p in ps]
+        opt.step()
+        norm = math.sqrt(sum(float(g.double().square().sum()) for g in gs))
+        assert abs(float(opt.grad_norm) / norm - 1) < 2 * U
+        for p, g, (p0, m0, v0) in zip(ps, gs, before):
+            p1, tp, *_ = _expected(p0, g, m0, v0, t, lr, *betas, eps, wd, min(1.0, 0.5 / (norm + 1e-6)))
+            _within(p, p1, tp + _store(p1, F32), ("p", t))

@@ -351,3 +351,19 @@ def test_one_row_with_any_stride_through_the_c_entry():
     check(lib.nsr_layer_norm_backward(ptr(dy), 0, ptr(x), 0, ptr(w), ptr(mean), ptr(rstd), ptr(dx0), ptr(dw0), ptr(db0), None, 1, 64,
                                       0, 0, stream_ptr()))
     assert all(torch.equal(p, q) for p, q in ((y, y0), (dx, dx0), (dw, dw0), (db, db0)))
+
+
+@pytest.mark.parametrize("dtype,width", [(F32, 8), (BF16, 16), (BF16, 9), (F32, 3)])
+def test_more_rows_than_workgroups_at_once(dtype, width):
+    """so many narrow rows that every workgroup walks several tiles"""
+    from nsr_hip import ops
+    rows = 4_300_001
+    x, w, b, dy = _inputs(rows, width, dtype, F32, 14)
+    y, mean, rstd = ops.layer_norm_forward(x, w, b)
+    want, tol = _reference(x, w, b, 1e-5)[:2]
+    _close(y, want, tol, "y")
+    dx, dw, db = ops.layer_norm_backward(dy, x, w, mean, rstd)
+    (r, t), (rw, tw), (rb, tb) = _reference_backward(dy, x, w, mean, rstd)
+    _close(dx, r, t, "dx")
+    _close(dw, rw, tw + _store(rw, F32), "dweight")
+    _close(db, rb, tb + _store(rb, F32), "dbias")
