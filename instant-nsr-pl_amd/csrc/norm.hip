@@ -79,6 +79,26 @@ __device__ __forceinline__ float pairwise(F f, int at = 0)
     else return pairwise<N / 2>(f, at) + pairwise<N / 2>(f, at + N / 2);
 }
 
+// 1 / sqrt(v) to 1 ulp; the instruction takes denormal numbers for zero
+__device__ __forceinline__ float inverse_sqrt(float v)
+{
+    const bool small = v < 0x1p-100f;
+    return __builtin_amdgcn_rsqf(small ? v * 0x1p100f : v) * (small ? 0x1p50f : 1.f);
+}
+
+// sum of f(k) g(k), k < N, in two chains of fma
+template <int N, class F, class H>
+__device__ __forceinline__ float dot(F f, H g)
+{
+    float a = f(0) * g(0), b = N > 1 ? f(1 % N) * g(1 % N) : 0.f;
+#pragma unroll
+    for (int k = 2; k < N; k += 2) {
+        a = fmaf(f(k), g(k), a);
+        b = fmaf(f(k + 1), g(k + 1), b);
+    }
+    return a + b;
+}
+
 // ---- vectors of a row ------------------------------------------------------------------------------------------------------
 template <class T> struct Vec16 { static constexpr int N = 16 / sizeof(T); };
 
@@ -117,7 +137,7 @@ __device__ __forceinline__ void store_vec(T *row, uint32_t col, uint32_t width, 
 //   BUFFER  rows at 4-byte addresses (fp32; 16 bits with even widths and strides): buffer instructions, where lanes outside the
 //           row and rows past the end have offsets past the buffer's end: loads give zero, stores do nothing;
 //   GLOBAL  16-bit rows at odd addresses: global instructions, which take any address; a lane outside the row repeats its last
-//           vector and a row past the end the last row, which stores what is stored there anyway;
+//           vector and a row past the end the last row, and neither stores;
 //   TINY    rows of less than a vector, element by element.
 // In the first two nothing branches around a load, in the first around a store either, and only so can the compiler count what
 // is outstanding: behind a branch it waits for everything, also for the loads of the next row and the stores of the last one
@@ -170,29 +190,34 @@ __device__ __forceinline__ Place place(uint32_t vector, uint32_t width)
     return {at, col - at};
 }
 
-// the rows of a tile, row0 .. row0 + groups - 1, in memory
-template <class T, Access A>
+// the rows of a tile, row0 .. row0 + GROUPS - 1, in memory; group_at = group * stride
+template <class T, Access A, int GROUPS>
 struct Rows {
     static constexpr int N = Vec16<T>::N;
     __amdgpu_buffer_rsrc_t buffer;
     T *row;
-    uint32_t group_at, width;  // (width 0: nothing to read or write, TINY)
+    uint32_t at0, width;  // (width 0: nothing to write, nor to read where the access is TINY)
 
-    __device__ __forceinline__ Rows(const T *p, uint64_t stride, uint64_t row0, uint32_t group, uint64_t rows, uint32_t width_)
-        : width(width_)
+    __device__ __forceinline__ Rows(const T *p, uint64_t stride, uint64_t row0, uint32_t group, uint64_t group_at, uint64_t rows,
+                                    uint32_t width_) : width(width_)
     {
         if constexpr (A == BUFFER) {
             buffer = rows_buffer(p + row0 * stride, (int64_t)(rows - row0), stride * sizeof(T), width_ * sizeof(T));
-            group_at = group * (uint32_t)stride;
+            at0 = (uint32_t)group_at;
         } else {
-            const uint64_t r = row0 + group;
-            if (A == TINY && r >= rows) width = 0;
-            row = const_cast<T *>(p) + (r < rows ? r : rows - 1) * stride;
+            const uint64_t r0 = row0 < rows ? row0 : rows - 1;  // (the same in every lane)
+            row = const_cast<T *>(p) + r0 * stride;
+            if constexpr (GROUPS > 1) {
+                const uint64_t last = rows - 1 - r0;
+                if (last >= GROUPS - 1) row += group_at;
+                else row += (group < last ? group : last) * stride;
+                if (row0 + group >= rows) width = 0;
+            }
         }
     }
     __device__ __forceinline__ Vec<T, N> load(const Place &p) const
     {
-        if constexpr (A == BUFFER) return buffer_load<Vec<T, N>>(buffer, p.twice < N ? (group_at + p.at) * sizeof(T) : OUTSIDE);
+        if constexpr (A == BUFFER) return buffer_load<Vec<T, N>>(buffer, p.twice < N ? (at0 + p.at) * sizeof(T) : OUTSIDE);
         if constexpr (A == TINY) return load_vec(row, p.at, width);
         Vec<T, N> v;
         __builtin_memcpy(&v, row + p.at, sizeof(v));
@@ -200,11 +225,23 @@ struct Rows {
     }
     __device__ __forceinline__ void store(const Place &p, const Vec<T, N> &v) const
     {
-        if constexpr (A == BUFFER) buffer_store(buffer, p.twice < N ? (group_at + p.at) * sizeof(T) : OUTSIDE, v);
+        if constexpr (A == BUFFER) buffer_store(buffer, p.twice < N ? (at0 + p.at) * sizeof(T) : OUTSIDE, v);
         else if constexpr (A == TINY) store_vec(row, p.at, width, v);
-        else if (p.twice < N) __builtin_memcpy(row + p.at, &v, sizeof(v));
+        else if (p.twice < N && (GROUPS == 1 || width)) __builtin_memcpy(row + p.at, &v, sizeof(v));
     }
 };
+
+// the vector, or zeros
+template <class V>
+__device__ __forceinline__ V kept(V v, bool keep)
+{
+    uint32_t u[sizeof(V) / 4];
+    __builtin_memcpy(u, &v, sizeof(v));
+#pragma unroll
+    for (uint32_t &w : u) w = keep ? w : 0u;
+    __builtin_memcpy(&v, u, sizeof(v));
+    return v;
+}
 
 // N affine parameters from `col` on, fp32 or of the rows' type; `none` where there are none
 template <class T, int N>
@@ -228,10 +265,12 @@ __device__ __forceinline__ void load_affine(const void *p, bool fp32, uint32_t c
 
 // ---- forward ---------------------------------------------------------------------------------------------------------------
 // Two sums over the row's registers (mean, then squares about it), one fma an element with weight and bias, which stay in
-// registers.  Bound by HBM: 2097152 x 64 fp16 in 94 us (5.7 TB/s), 8192 x 4096 bf16 in 25 us (5.3 TB/s).  Groups of more than a wave load the next row while they work on one; smaller ones
-// have enough waves without (2097152 x 64 fp16: 94 us without, 101 us with).
+// registers.  Bound by HBM: 2097152 x 64 fp16 in 94 us (5.7 TB/s), 8192 x 4096 bf16 in 22 us (6.0 TB/s).  Groups of more than
+// a wave load the next row while they work on one; smaller ones have enough waves without (2097152 x 64 fp16: 94 us without,
+// 101 us with).  16-bit rows of 256 threads and more are held to 64 registers, 8 waves: with the 66 that the compiler would take
+// a CU holds one workgroup of 1024 threads in place of two (6709 x 5001 bf16: 32 us, and 39 without).
 template <class T, int G, int ITER, Access A>
-__global__ void __launch_bounds__(G > 256 ? G : 256)
+__global__ void __launch_bounds__(G > 256 ? G : 256, sizeof(T) == 2 && G >= 256 && ITER == 1 ? 8 : 1)
 k_ln_forward(const T *__restrict__ x, uint64_t xs, const void *__restrict__ w, const void *__restrict__ b, int affine_fp32,
              T *__restrict__ y, float *__restrict__ mean, float *__restrict__ rstd, uint64_t rows, uint32_t width,
              float inv_width, float eps)
@@ -240,10 +279,11 @@ k_ln_forward(const T *__restrict__ x, uint64_t xs, const void *__restrict__ w, c
     __shared__ float lds[G > 64 ? 32 : 1];
     int turn = 0;
     const uint32_t lane = threadIdx.x % G, group = threadIdx.x / G;
+    const uint64_t x_at = group * xs, y_at = (uint64_t)group * width;
     const bool covered = width == (uint32_t)(G * N * ITER);
     Vec<T, N> raw[ITER];
     auto load_row = [&](uint64_t tile) {
-        const Rows<T, A> from(x, xs, tile * GROUPS, group, rows, width);
+        const Rows<T, A, GROUPS> from(x, xs, tile * GROUPS, group, x_at, rows, width);
 #pragma unroll
         for (int i = 0; i < ITER; ++i) raw[i] = from.load(place<N, A>(i * G + lane, width));
     };
@@ -279,12 +319,12 @@ k_ln_forward(const T *__restrict__ x, uint64_t xs, const void *__restrict__ w, c
         for (int i = 0; i < ITER; ++i) {
 #pragma unroll
             for (int k = 0; k < N; ++k) v[i][k] -= mu;
-            if (covered) t[0] += pairwise<N>([&](int k) { return v[i][k] * v[i][k]; });
-            else t[0] += pairwise<N>([&](int k) { return counts(i, k) ? v[i][k] * v[i][k] : 0.f; });
+            if (covered) t[0] += dot<N>([&](int k) { return v[i][k]; }, [&](int k) { return v[i][k]; });
+            else t[0] += dot<N>([&](int k) { return counts(i, k) ? v[i][k] : 0.f; }, [&](int k) { return v[i][k]; });
         }
         group_sum<G>(t, lds, turn);
-        const float rs = 1.f / sqrtf(t[0] * inv_width + eps);
-        const Rows<T, A> to(y, width, row0, group, rows, width);
+        const float rs = inverse_sqrt(t[0] * inv_width + eps);
+        const Rows<T, A, GROUPS> to(y, width, row0, group, y_at, rows, width);
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
             Vec<T, N> o;
@@ -323,7 +363,7 @@ k_ln_forward_long(const T *__restrict__ x, uint64_t xs, const void *__restrict__
             t[0] += pairwise<N>([&](int k) { const float d = c + k < width ? (float)v.e[k] - mu : 0.f; return d * d; });
         }
         group_sum<1024>(t, lds, turn);
-        const float rs = 1.f / sqrtf(t[0] * inv_width + eps);
+        const float rs = inverse_sqrt(t[0] * inv_width + eps);
         for (uint64_t c = threadIdx.x * N; c < width; c += 1024 * N) {
             Vec<T, N> v = load_vec(xr, (uint32_t)c, width);
             float wv[N], bv[N];
@@ -372,27 +412,28 @@ k_ln_backward(const T *__restrict__ dy, uint64_t dys, const T *__restrict__ x, u
     __shared__ float sums[SETS > 1 ? SETS * G * N : 1];
     int turn = 0;
     const uint32_t lane = threadIdx.x % G, group = threadIdx.x / G;
-    // no element counts twice: what lies outside the row is zero, or nothing does
-    const bool whole = A == TINY || (A == BUFFER && width % N == 0) || width == (uint32_t)(G * N * ITER);
+    const uint64_t x_at = group * xs, d_at = group * dys, to_at = (uint64_t)group * width;
+    // no element counts twice: what lies outside the row is zero
+    const bool whole = A == TINY || (A == BUFFER && width % N == 0);
     Vec<T, N> xr[ITER], dr[ITER];
     float mu, rs;
     auto load_row = [&](uint64_t tile) {
         const uint64_t row0 = tile * GROUPS;
         const int64_t left = (int64_t)(rows - row0);
-        const Rows<T, A> from_x(x, xs, row0, group, rows, width), from_d(dy, dys, row0, group, rows, width);
+        const Rows<T, A, GROUPS> from_x(x, xs, row0, group, x_at, rows, width), from_d(dy, dys, row0, group, d_at, rows, width);
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
             const Place p = place<N, A>(i * G + lane, width);
             xr[i] = from_x.load(p);
             dr[i] = from_d.load(p);
         }
-        if constexpr (A == BUFFER) {
-            mu = buffer_load<float>(rows_buffer(mean + row0, left, 4, 4), group * 4);
-            rs = buffer_load<float>(rows_buffer(rstd + row0, left, 4, 4), group * 4);
-        } else {
-            const uint64_t r = group < left ? row0 + group : rows - 1;
+        if constexpr (GROUPS == 1) {
+            const uint64_t r = row0 < rows ? row0 : rows - 1;
             mu = mean[r];
             rs = rstd[r];
+        } else {
+            mu = buffer_load<float>(rows_buffer(mean + row0, left, 4, 4), group * 4);
+            rs = buffer_load<float>(rows_buffer(rstd + row0, left, 4, 4), group * 4);
         }
     };
     load_row(blockIdx.x);
@@ -410,12 +451,14 @@ k_ln_backward(const T *__restrict__ dy, uint64_t dys, const T *__restrict__ x, u
         float h[ITER][N], g[ITER][N], t[2] = {0.f, 0.f};
         const float rs0 = rs;
 #pragma unroll
-        for (int i = 0; i < ITER; ++i)
+        for (int i = 0; i < ITER; ++i) {
+            if constexpr (A == GLOBAL && GROUPS > 1) dr[i] = kept(dr[i], row < rows);  // (a row past the end came as the last one)
 #pragma unroll
             for (int k = 0; k < N; ++k) {
                 g[i][k] = (float)dr[i].e[k];
                 h[i][k] = ((float)xr[i].e[k] - mu) * rs0;
             }
+        }
         if constexpr (HELD) load_row(tile + gridDim.x);
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
@@ -426,29 +469,31 @@ k_ln_backward(const T *__restrict__ dy, uint64_t dys, const T *__restrict__ x, u
             }
 #pragma unroll
             for (int k = 0; k < N; ++k) {
-                const float d = A == GLOBAL && row >= rows ? 0.f : g[i][k];  // (a row that repeats the last one)
-                sw[i][k] = fmaf(d, h[i][k], sw[i][k]);
-                sb[i][k] += d;
+                sw[i][k] = fmaf(g[i][k], h[i][k], sw[i][k]);
+                sb[i][k] += g[i][k];
                 g[i][k] *= wv[HELD ? i : 0][k];
             }
-            if (whole) {
+            if (A != GLOBAL && whole) {  // (16-bit rows at odd addresses are never whole)
                 t[0] += pairwise<N>([&](int k) { return g[i][k]; });
-                t[1] += pairwise<N>([&](int k) { return g[i][k] * h[i][k]; });
+                t[1] += dot<N>([&](int k) { return g[i][k]; }, [&](int k) { return h[i][k]; });
             } else {
                 const int twice = (int)place<N, A>(i * G + lane, width).twice;
-                t[0] += pairwise<N>([&](int k) { return k >= twice ? g[i][k] : 0.f; });
-                t[1] += pairwise<N>([&](int k) { return k >= twice ? g[i][k] * h[i][k] : 0.f; });
+                float once[N];
+#pragma unroll
+                for (int k = 0; k < N; ++k) once[k] = k >= twice ? g[i][k] : 0.f;
+                t[0] += pairwise<N>([&](int k) { return once[k]; });
+                t[1] += dot<N>([&](int k) { return once[k]; }, [&](int k) { return h[i][k]; });
             }
         }
         if (dx) {  // (the same for every thread)
             group_sum<G>(t, lds, turn);
             const float a = t[0] * inv_width, c = t[1] * inv_width;
-            const Rows<T, A> to(dx, width, row0, group, rows, width);
+            const Rows<T, A, GROUPS> to(dx, width, row0, group, to_at, rows, width);
 #pragma unroll
             for (int i = 0; i < ITER; ++i) {
                 Vec<T, N> o;
 #pragma unroll
-                for (int k = 0; k < N; ++k) o.e[k] = (T)(rs0 * (g[i][k] - a - h[i][k] * c));
+                for (int k = 0; k < N; ++k) o.e[k] = (T)(rs0 * fmaf(-h[i][k], c, g[i][k] - a));
                 to.store(place<N, A>(i * G + lane, width), o);
             }
         }

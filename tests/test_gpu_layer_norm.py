@@ -367,3 +367,22 @@ def test_more_rows_than_workgroups_at_once(dtype, width):
     _close(dx, r, t, "dx")
     _close(dw, rw, tw + _store(rw, F32), "dweight")
     _close(db, rb, tb + _store(rb, F32), "dbias")
+
+
+@pytest.mark.parametrize("width", [64, 65, 4096])
+def test_variances_below_the_smallest_normal_number(width):
+    from nsr_hip import ops
+
+    x = torch.randn(9, width, generator=torch.Generator(device="cuda").manual_seed(5), device="cuda") * 1e-20
+    y, mean, rstd = ops.layer_norm_forward(x, eps=0.0)
+    x64 = x.double()
+    mean64 = x64.mean(-1, keepdim=True)
+    var = (x64 - mean64).square().mean(-1, keepdim=True)  # about 1e-40
+    # each square and the mean of them is rounded to a multiple of 2^-149, so the variance is off by at most 2^-149 more
+    # than the roundings and the mean's error that rows of any size have; rstd by half of that relative to itself
+    k = math.ceil(width / 64) + 6
+    d_mean = (k + 2) * U * x64.abs().mean(-1, keepdim=True)
+    rel = (k + 10) * U + 2.0 ** -149 / var + d_mean.square() / var
+    assert ((rstd.double()[:, None] - var.rsqrt()).abs() <= var.rsqrt() * (rel + 4 * U)).all()
+    h = (x64 - mean64) * var.rsqrt()
+    assert ((y.double() - h).abs() <= var.rsqrt() * d_mean * (1 + rel) + h.abs() * (rel + 8 * U)).all()
