@@ -413,7 +413,7 @@ k_ln_backward(const T *__restrict__ dy, uint64_t dys, const T *__restrict__ x, u
     int turn = 0;
     const uint32_t lane = threadIdx.x % G, group = threadIdx.x / G;
     const uint64_t x_at = group * xs, d_at = group * dys, to_at = (uint64_t)group * width;
-    // no element counts twice: what lies outside the row is zero
+    // no element counts twice: what lies outside the row is zero (not asked for GLOBAL, whose widths are odd for the most part)
     const bool whole = A == TINY || (A == BUFFER && width % N == 0);
     Vec<T, N> xr[ITER], dr[ITER];
     float mu, rs;
@@ -473,7 +473,7 @@ k_ln_backward(const T *__restrict__ dy, uint64_t dys, const T *__restrict__ x, u
                 sb[i][k] += g[i][k];
                 g[i][k] *= wv[HELD ? i : 0][k];
             }
-            if (A != GLOBAL && whole) {  // (16-bit rows at odd addresses are never whole)
+            if (A != GLOBAL && whole) {
                 t[0] += pairwise<N>([&](int k) { return g[i][k]; });
                 t[1] += dot<N>([&](int k) { return g[i][k]; }, [&](int k) { return h[i][k]; });
             } else {

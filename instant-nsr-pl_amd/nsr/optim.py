@@ -10,6 +10,8 @@ from nsr_hip.ops import DTYPE_CODES, timed
 
 F32, F8 = torch.float32, torch.float8_e4m3fn
 _DESCRIPTOR = np.dtype(NsrAdamwTensor)
+# (of a list by map: the host side of a step of many tensors is these)
+_address, _size, _contiguous = torch.Tensor.data_ptr, torch.Tensor.nbytes.__get__, torch.Tensor.is_contiguous
 BLOCK = 256  # elements under one scale of the 8-bit moments (csrc/optim.hip); every tensor's moments start at a multiple of it
 
 
@@ -226,13 +228,17 @@ class AdamW(torch.optim.Optimizer):
         """this step's addresses in the descriptors; (host array, count, live parameters, tensors to keep until the launch)"""
         f, ps = self._fields, self._ps
         grads = [p.grad for p in ps]
-        addresses = [p.data_ptr() for p in ps]
+        addresses = list(map(_address, ps))
         if addresses != self._addresses:
             self._check_moved()
             self._addresses = addresses
             f["params"] = addresses
         keep = []
-        if not self._all_contiguous or any([g is None or not g.is_contiguous() for g in grads]):
+        try:
+            whole = self._all_contiguous and all(map(_contiguous, grads))
+        except TypeError:  # (a gradient is None)
+            whole = False
+        if not whole:
             for i, (p, g) in enumerate(zip(ps, grads)):
                 if g is None:
                     continue
@@ -250,8 +256,8 @@ class AdamW(torch.optim.Optimizer):
                     f["grad"][i] = grads[i].data_ptr()
                 some = f[live]  # (a copy)
                 return some.ctypes.data, len(live), [ps[i] for i in live], (keep, some)
-        self._check_sizes([g.nbytes for g in grads], self._nbytes)
-        f["grad"] = [g.data_ptr() for g in grads]
+        self._check_sizes(list(map(_size, grads)), self._nbytes)
+        f["grad"] = list(map(_address, grads))
         return self._desc, len(ps), ps, keep
 
     @staticmethod
