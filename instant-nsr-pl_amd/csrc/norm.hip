@@ -265,7 +265,7 @@ __device__ __forceinline__ void load_affine(const void *p, bool fp32, uint32_t c
 
 // ---- forward ---------------------------------------------------------------------------------------------------------------
 // Two sums over the row's registers (mean, then squares about it), one fma an element with weight and bias, which stay in
-// registers.  Bound by HBM: 2097152 x 64 fp16 in 94 us (5.7 TB/s), 8192 x 4096 bf16 in 22 us (6.0 TB/s).  Groups of more than
+// registers.  Bound by HBM: 2097152 x 64 fp16 in 94 us (5.7 TB/s), 8192 x 4096 bf16 in 24 us (5.6 TB/s).  Groups of more than
 // a wave load the next row while they work on one; smaller ones have enough waves without (2097152 x 64 fp16: 94 us without,
 // 101 us with).  16-bit rows of 256 threads and more are held to 64 registers, 8 waves: with the 66 that the compiler would take
 // a CU holds one workgroup of 1024 threads in place of two (6709 x 5001 bf16: 32 us, and 39 without).
