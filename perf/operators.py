@@ -27,19 +27,13 @@ LEAST = 2.0 ** -100      # a block's largest magnitude counts as at least this m
 DTYPES = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}
 
 
-_modules = []
-
-
 def _framework():
-    """the framework's modules, imported once (a program does not look them up again in every pass)"""
-    if not _modules:
-        at = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "instant-nsr-pl_amd")
-        if at not in sys.path:
-            sys.path.insert(0, at)
-        from nsr import optim
-        from nsr_hip import ops
-        _modules.extend((optim, ops))
-    return _modules
+    at = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "instant-nsr-pl_amd")
+    if at not in sys.path:
+        sys.path.insert(0, at)
+    from nsr import optim
+    from nsr_hip import ops
+    return optim, ops
 
 
 # ---------------------------------------------------------------------------------------------------------------------
