@@ -12,6 +12,7 @@ F32, F8 = torch.float32, torch.float8_e4m3fn
 _DESCRIPTOR = np.dtype(NsrAdamwTensor)
 # (of a list by map: the host side of a step of many tensors is these)
 _address, _size, _contiguous = torch.Tensor.data_ptr, torch.Tensor.nbytes.__get__, torch.Tensor.is_contiguous
+_dtype, _device = torch.Tensor.dtype.__get__, torch.Tensor.get_device
 BLOCK = 256  # elements under one scale of the 8-bit moments (csrc/optim.hip); every tensor's moments start at a multiple of it
 
 
@@ -102,7 +103,7 @@ class AdamW(torch.optim.Optimizer):
         self._group_of = [i for _, i in items]
         self._all_contiguous = all(p.is_contiguous() for p in self._ps)
         self._addresses = [p.data_ptr() for p in self._ps]
-        self._nbytes = [p.nbytes for p in self._ps]
+        self._kinds = [list(map(of, self._ps)) for of in (_size, _dtype, _device)]
         self._bits = [8 if self.state_bits == 8 and p.numel() >= self.min_8bit_size else 32 for p in self._ps]
         n = np.array([p.numel() for p in self._ps], dtype=np.int64)
         eight = np.array([b == 8 for b in self._bits])
@@ -239,32 +240,35 @@ class AdamW(torch.optim.Optimizer):
         except TypeError:  # (a gradient is None)
             whole = False
         if not whole:
-            for i, (p, g) in enumerate(zip(ps, grads)):
-                if g is None:
-                    continue
-                if g.layout is not torch.strided:
-                    raise NsrError(f"AdamW: a gradient of layout {g.layout} is not supported")
+            live = [i for i, g in enumerate(grads) if g is not None]
+            for i in live:
+                if grads[i].layout is not torch.strided:
+                    raise NsrError(f"AdamW: a gradient of layout {grads[i].layout} is not supported")
+            self._check_kinds([grads[i] for i in live], [[kind[i] for i in live] for kind in self._kinds])
+            for i in live:
+                p, g = ps[i], grads[i]
                 if g.stride() != p.stride() and p.numel():  # in the parameter's order of elements
                     grads[i] = torch.empty_strided(p.shape, p.stride(), dtype=p.dtype, device=p.device)
                     with torch.no_grad():
                         grads[i].copy_(g)
             keep = grads
-            live = [i for i, g in enumerate(grads) if g is not None]
-            self._check_sizes([grads[i].nbytes for i in live], [self._nbytes[i] for i in live])
             if len(live) < len(ps):
                 for i in live:
                     f["grad"][i] = grads[i].data_ptr()
                 some = f[live]  # (a copy)
                 return some.ctypes.data, len(live), [ps[i] for i in live], (keep, some)
-        self._check_sizes(list(map(_size, grads)), self._nbytes)
+        else:
+            self._check_kinds(grads, self._kinds)
         f["grad"] = list(map(_address, grads))
         return self._desc, len(ps), ps, keep
 
     @staticmethod
-    def _check_sizes(got, want):
-        # torch sees to it for ``p.grad = g``, but not for ``p.grad.data = g`` or a ``grad_dtype`` of its own
-        if got != want:
-            raise NsrError("AdamW: a gradient has another size or type than its parameter")
+    def _check_kinds(grads, kinds):
+        # the kernel reads a gradient by its address with the parameter's type.  torch sees to it for ``p.grad = g``, but not for
+        # ``p.grad.data = g`` or a ``grad_dtype`` of its own
+        sizes, dtypes, devices = kinds
+        if list(map(_size, grads)) != sizes or list(map(_dtype, grads)) != dtypes or list(map(_device, grads)) != devices:
+            raise NsrError("AdamW: a gradient has another size, type or device than its parameter")
 
     def _check_moved(self):
         """parameters whose memory was replaced (``p.data = ...``) still have the layout that the moments were made for"""

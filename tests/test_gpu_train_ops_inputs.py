@@ -1,0 +1,39 @@
+"""Inputs that the training operators (``nsr.optim.AdamW``, layer norm) refuse or have to see, on the GPU."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def _bytes(opt):
+    return [t.clone().view(torch.uint8) for t in (*opt.flat32.values(), *opt.flat8.values())]
+
+
+@pytest.mark.parametrize("kind,other", [(F16, BF16), (BF16, F16)])
+@pytest.mark.parametrize("bits,clip", [(32, None), (32, 1.0), (8, None)])
+@pytest.mark.parametrize("strided", [False, True])
+@pytest.mark.parametrize("beside_none", [False, True])
+def test_gradient_of_the_other_16_bit_type_is_refused(kind, other, bits, clip, strided, beside_none):
+    """refused before any launch: parameters, moments and the step count stay"""
+    import nsr.optim
+    from nsr_hip import NsrError
+    ps = [torch.nn.Parameter(torch.randn(70, 60, device="cuda").to(kind)) for _ in range(2)]
+    opt = nsr.optim.AdamW(ps, lr=0.1, state_bits=bits, min_8bit_size=0, max_grad_norm=clip)
+    for p in ps:
+        p.grad = torch.randn(70, 60, device="cuda").to(kind)
+    opt.step()
+    before, moments = [p.detach().clone() for p in ps], _bytes(opt)
+    if beside_none:
+        ps[1].grad = None
+    g = torch.randn(70, 60, device="cuda").to(other)
+    ps[0].grad.data = g.t().contiguous().t() if strided else g
+    with pytest.raises(NsrError, match="another size, type or device"):
+        opt.step()
+    ps[0].grad = None
+    ps[0].grad_dtype = other
+    ps[0].grad = g
+    with pytest.raises(NsrError, match="another size, type or device"):
+        opt.step()
+    assert all(torch.equal(p, q) for p, q in zip(ps, before)) and opt.taken_steps() == 1
+    assert all(torch.equal(a, b) for a, b in zip(_bytes(opt), moments))

@@ -1,0 +1,54 @@
+"""Inputs of the training operators (``nsr.optim.AdamW``, layer norm) that are refused before anything reaches a kernel, on the
+CPU."""
+import numpy as np
+import pytest
+import torch
+
+
+def _gathering(p):
+    """an optimizer of one tensor as far as the gathering of its gradients goes (construction needs a GPU)"""
+    from nsr import optim
+    opt = object.__new__(optim.AdamW)
+    opt._ps, opt._addresses, opt._all_contiguous = [p], [p.data_ptr()], p.is_contiguous()
+    opt._kinds = [[of(p)] for of in (optim._size, optim._dtype, optim._device)]
+    opt._desc = (optim.NsrAdamwTensor * 1)()
+    opt._fields = np.frombuffer(opt._desc, dtype=optim._DESCRIPTOR)
+    return opt
+
+
+@pytest.mark.parametrize("kind,other,by", [(torch.float16, torch.bfloat16, "data"), (torch.bfloat16, torch.float16, "data"),
+                                           (torch.float32, torch.int32, "data"), (torch.float16, torch.bfloat16, "grad_dtype"),
+                                           (torch.bfloat16, torch.float16, "grad_dtype")])
+@pytest.mark.parametrize("strided", [False, True])
+def test_gradient_of_another_type_of_the_same_size(kind, other, strided, by):
+    """the kernel reads a gradient with its parameter's type: one of another type is refused in every layout, none is converted"""
+    from nsr_hip import NsrError
+    p = torch.nn.Parameter(torch.zeros(4, 6, dtype=kind))
+    opt = _gathering(p)
+    g = torch.ones(4, 6, dtype=other)
+    g = g.t().contiguous().t() if strided else g
+    if by == "data":
+        p.grad = torch.zeros(4, 6, dtype=kind)
+        p.grad.data = g
+    else:
+        p.grad_dtype = other
+        p.grad = g
+    assert p.grad.dtype == other and p.grad.nbytes == p.nbytes and p.grad.is_contiguous() != strided
+    with pytest.raises(NsrError, match="another size, type or device"):
+        opt._gather()
+    p.grad = None
+    p.grad_dtype = kind
+    p.grad = torch.ones(4, 6, dtype=kind)
+    assert opt._gather()[1] == 1 and opt._fields["grad"][0] == p.grad.data_ptr()
+
+
+@pytest.mark.parametrize("strided", [False, True])
+def test_gradient_on_another_device(strided):
+    """an address in another device's memory reaches no kernel (the optimizer's own device is a GPU, the gradient is not there)"""
+    from nsr_hip import NsrError
+    p = torch.nn.Parameter(torch.zeros(4, 6))
+    opt = _gathering(p)
+    opt._kinds[2] = [0]
+    p.grad = torch.ones(6, 4).t() if strided else torch.ones(4, 6)
+    with pytest.raises(NsrError, match="another size, type or device"):
+        opt._gather()
