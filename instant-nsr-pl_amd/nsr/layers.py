@@ -10,7 +10,7 @@ class LayerNorm(nn.Module):
     """Layer norm over the last axis (``torch.nn.LayerNorm``'s formula, state-dict keys and defaults for one axis).
 
     Inputs are float32, float16 or bfloat16 on the GPU; ``weight`` / ``bias`` are float32 unless ``dtype`` names the inputs'
-    type.  The output has the input's type.  Differentiable once."""
+    type.  The output has the input's type.  Differentiable once, in reverse mode."""
 
     def __init__(self, width, eps=1e-5, elementwise_affine=True, bias=True, device=None, dtype=torch.float32):
         super().__init__()

@@ -9,7 +9,7 @@ import time
 import os
 
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import NsrError, check, device_guard, lib, ptr, stream_ptr
@@ -845,8 +845,18 @@ def _rows(t, width):
     return t.contiguous(), t.numel() // width, width
 
 
+def _no_tangents(name, *tensors):
+    """refuses forward mode: a dual tensor has its primal's address, the kernels' results would come back without a tangent"""
+    if forward_ad._current_level < 0:  # (outside of every dual_level there are none; asking each tensor costs 1 us a call)
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None and torch._C._is_fwd_grad_enabled():
+            raise NsrError(f"{name}: forward mode (a tangent) is not supported")
+
+
 def _ln_check(x, weight, bias):
     """refuses what the kernels do not take; the type of the affine parameters (the input's without any)"""
+    _no_tangents("layer_norm", x, weight, bias)
     if x.dtype not in DTYPE_CODES:
         raise NsrError(f"layer_norm: expected a float32/float16/bfloat16 tensor, got {x.dtype}")
     if not x.is_cuda:
@@ -905,6 +915,7 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5):
 def layer_norm_backward(dy, x, weight, mean, rstd, want_dx=True, want_dweight=True, want_dbias=True, affine_dtype=None):
     """``(dx, dweight, dbias)`` of ``layer_norm_forward`` (None where not wanted).  ``dweight`` / ``dbias`` have ``weight``'s type
     (``affine_dtype``, by default ``x``'s, without one); sums over the rows are in float32 and the same for the same inputs."""
+    _no_tangents("layer_norm_backward", dy, mean, rstd)
     affine = _ln_check(x, weight, None)
     if weight is None and affine_dtype is not None:
         if affine_dtype not in (F32, x.dtype):
@@ -954,10 +965,17 @@ class _LayerNorm(Function):
         return dx, dw, db, None
 
 
+def _ln_wants_grad(x, weight, bias):
+    if not torch.is_grad_enabled() or not (x.requires_grad or (weight is not None and weight.requires_grad) or
+                                           (bias is not None and bias.requires_grad)):
+        return False
+    _no_tangents("layer_norm", x, weight, bias)  # (the tangents are out of sight inside the autograd function)
+    return True
+
+
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
-    """layer norm over the last axis, differentiable once (a second differentiation raises); types and shapes as in
-    ``layer_norm_forward``.  Nothing but ``y`` is written where no gradient is wanted."""
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
-                                    (bias is not None and bias.requires_grad)):
+    """layer norm over the last axis, differentiable once in reverse mode (a second differentiation raises, and so does forward
+    mode); types and shapes as in ``layer_norm_forward``.  Nothing but ``y`` is written where no gradient is wanted."""
+    if _ln_wants_grad(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, float(eps))
     return _layer_norm(x, weight, bias, eps, False)[0]

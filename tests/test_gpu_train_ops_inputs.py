@@ -37,3 +37,22 @@ def test_gradient_of_the_other_16_bit_type_is_refused(kind, other, bits, clip, s
         opt.step()
     assert all(torch.equal(p, q) for p, q in zip(ps, before)) and opt.taken_steps() == 1
     assert all(torch.equal(a, b) for a, b in zip(_bytes(opt), moments))
+
+
+def test_layer_norm_refuses_forward_mode():
+    from torch.autograd import forward_ad
+    from nsr.layers import LayerNorm
+    from nsr_hip import NsrError, ops
+    x, t = torch.randn(2, 5, 16, device="cuda")
+    ln = LayerNorm(16).cuda()
+    with forward_ad.dual_level():
+        xd = forward_ad.make_dual(x, t)
+        for call in (lambda: ops.layer_norm(xd), lambda: ops.layer_norm_forward(xd), lambda: ln(xd),
+                     lambda: ops.layer_norm(x, forward_ad.make_dual(x[0], t[0]))):
+            with pytest.raises(NsrError, match="forward mode"):
+                call()
+        with torch.no_grad(), pytest.raises(NsrError, match="forward mode"):
+            ln(xd)
+        assert ops.layer_norm(x).shape == x.shape  # (no tangent among the inputs)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(ops.layer_norm, (x,), (t,))

@@ -52,3 +52,22 @@ def test_gradient_on_another_device(strided):
     p.grad = torch.ones(6, 4).t() if strided else torch.ones(4, 6)
     with pytest.raises(NsrError, match="another size, type or device"):
         opt._gather()
+
+
+@pytest.mark.parametrize("which", ["x", "weight", "bias", "dy", "mean", "rstd"])
+def test_layer_norm_refuses_tangents(which):
+    """forward mode: a result without its tangent would be a derivative of zero"""
+    from torch.autograd import forward_ad
+    from nsr_hip import NsrError, ops
+    with forward_ad.dual_level():
+        dual = lambda name, *shape: (forward_ad.make_dual(torch.ones(*shape), torch.ones(*shape)) if name == which  # noqa: E731
+                                     else torch.ones(*shape))
+        x, w, b, dy, mean, rstd = (dual(*a) for a in (("x", 3, 8), ("weight", 8), ("bias", 8), ("dy", 3, 8), ("mean", 3), ("rstd", 3)))
+        calls = [lambda: ops.layer_norm_backward(dy, x, w, mean, rstd)] if which != "bias" else []
+        if which in ("x", "weight", "bias"):
+            leaf = torch.ones(8, requires_grad=True)
+            calls += [lambda: ops.layer_norm(x, w, b), lambda: ops.layer_norm_forward(x, w, b)]
+            calls += [lambda: ops.layer_norm(x, leaf, b)] if which != "weight" else [lambda: ops.layer_norm(x, w, leaf)]
+        for call in calls:
+            with pytest.raises(NsrError, match="forward mode"):
+                call()
