@@ -908,13 +908,17 @@ def _layer_norm(x, weight, bias, eps, want_stats):
 
 def layer_norm_forward(x, weight=None, bias=None, eps=1e-5):
     """``(y, mean, rstd)``: ``x`` [..., width] normalised over its last axis, times ``weight`` plus ``bias`` ([width], float32 or
-    ``x``'s type; either may be None), and the rows' statistics in float32 (``x.shape[:-1]``) for ``layer_norm_backward``"""
+    ``x``'s type; either may be None), and the rows' statistics in float32 (``x.shape[:-1]``) for ``layer_norm_backward``.
+    ``y`` is differentiable as in ``layer_norm``; no gradient flows through the statistics."""
+    if _ln_wants_grad(x, weight, bias):
+        return _LayerNorm.apply(x, weight, bias, float(eps))
     return _layer_norm(x, weight, bias, eps, True)
 
 
 def layer_norm_backward(dy, x, weight, mean, rstd, want_dx=True, want_dweight=True, want_dbias=True, affine_dtype=None):
     """``(dx, dweight, dbias)`` of ``layer_norm_forward`` (None where not wanted).  ``dweight`` / ``dbias`` have ``weight``'s type
-    (``affine_dtype``, by default ``x``'s, without one); sums over the rows are in float32 and the same for the same inputs."""
+    (``affine_dtype``, by default ``x``'s, without one); sums over the rows are in float32 and the same for the same inputs.
+    They are results, detached from every graph: nothing differentiates through this call."""
     _no_tangents("layer_norm_backward", dy, mean, rstd)
     affine = _ln_check(x, weight, None)
     if weight is None and affine_dtype is not None:
@@ -953,12 +957,16 @@ class _LayerNorm(Function):
     def forward(ctx, x, weight, bias, eps):
         y, mean, rstd = _layer_norm(x, weight, bias, eps, True)
         ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.mark_non_differentiable(mean, rstd)
+        ctx.set_materialize_grads(False)  # (or zeros would be made for the statistics)
         ctx.bias_dtype = None if bias is None else bias.dtype
-        return y
+        return y, mean, rstd
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, dy):
+    def backward(ctx, dy, *_):
+        if dy is None:
+            return None, None, None, None
         x, weight, mean, rstd = ctx.saved_tensors
         want = ctx.needs_input_grad
         dx, dw, db = layer_norm_backward(dy, x, weight, mean, rstd, want[0], want[1], want[2], affine_dtype=ctx.bias_dtype)
@@ -977,5 +985,5 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """layer norm over the last axis, differentiable once in reverse mode (a second differentiation raises, and so does forward
     mode); types and shapes as in ``layer_norm_forward``.  Nothing but ``y`` is written where no gradient is wanted."""
     if _ln_wants_grad(x, weight, bias):
-        return _LayerNorm.apply(x, weight, bias, float(eps))
+        return _LayerNorm.apply(x, weight, bias, float(eps))[0]
     return _layer_norm(x, weight, bias, eps, False)[0]

@@ -56,3 +56,23 @@ def test_layer_norm_refuses_forward_mode():
         assert ops.layer_norm(x).shape == x.shape  # (no tangent among the inputs)
     with pytest.raises(RuntimeError):
         torch.func.jvp(ops.layer_norm, (x,), (t,))
+
+
+def test_layer_norm_forward_keeps_the_graph():
+    """y of the statistics form has the gradients of layer_norm, whichever inputs want them"""
+    from nsr_hip import ops
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, w, b, dy = (torch.randn(*s, generator=g, device="cuda") for s in ((40, 24), (24,), (24,), (40, 24)))
+    for wants in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 1, 1)):
+        grads = []
+        for f in (ops.layer_norm, lambda *a: ops.layer_norm_forward(*a)[0]):
+            leaves = [t.clone().requires_grad_(bool(k)) for t, k in zip((x, w, b), wants)]
+            y = f(*leaves)
+            y.backward(dy)
+            grads.append([y.detach()] + [t.grad for t in leaves if t.requires_grad])
+        assert len(grads[0]) == 1 + sum(wants) and all(torch.equal(p, q) for p, q in zip(*grads))
+    y, mean, rstd = ops.layer_norm_forward(x.clone().requires_grad_(), w, b)
+    assert y.requires_grad and not mean.requires_grad and not rstd.requires_grad
+    assert all(torch.equal(p, q) for p, q in zip((y, mean, rstd), ops.layer_norm_forward(x, w, b)))
+    with torch.no_grad():
+        assert not ops.layer_norm_forward(x.clone().requires_grad_(), w, b)[0].requires_grad
