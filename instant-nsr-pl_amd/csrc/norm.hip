@@ -45,29 +45,40 @@ __device__ __forceinline__ float lanes_sum(float v)
     return v;
 }
 
-// sums of N values over G threads; above a wave through LDS (`turn` alternates between two buffers, so that one barrier is
-// enough: a buffer is written again only behind the barrier of the other one)
+// sums of N values (1 or 2) over G threads.  Two values share the way: a swap of half groups leaves the one's partial sums in the
+// lower half and the other's in the upper, so that one register goes through the rest.  Above a wave through LDS (`turn` alternates
+// between two buffers, so that one barrier is enough: a buffer is written again only behind the barrier of the other one), where a
+// lane reads one wave's sum and lane moves add them.
 template <int G, int N>
 __device__ __forceinline__ void group_sum(float (&v)[N], float *lds, int &turn)
 {
+    static_assert(N == 1 || N == 2, "one value or two");
+    constexpr bool HALVES = N == 2 && G >= 32;
+    constexpr int HALF = G == 32 ? 16 : 32;
+    auto swapped = [](float a, float b) {
+        if constexpr (G == 32) return __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+        else return __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    };
+    if constexpr (HALVES) {
+        const auto r = swapped(v[0], v[N - 1]);
+        v[0] = lanes_sum<HALF>(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+    } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = lanes_sum<(G < 64 ? G : 64)>(v[i]);
+        for (int i = 0; i < N; ++i) v[i] = lanes_sum<(G < 64 ? G : 64)>(v[i]);
+    }
     if constexpr (G > 64) {
-        constexpr int WAVES = G / 64;
+        constexpr int WAVES = G / 64, LANES = 64 / N;  // (lanes that hold the same value)
         float *mine = lds + turn * (16 * N);
         turn ^= 1;
-        const uint32_t wave = threadIdx.x >> 6, first = wave / WAVES * WAVES;
-        if ((threadIdx.x & 63) == 0)
-#pragma unroll
-            for (int i = 0; i < N; ++i) mine[wave * N + i] = v[i];
+        const uint32_t wave = threadIdx.x >> 6, which = N == 1 ? 0 : threadIdx.x >> 5 & 1, first = wave / WAVES * WAVES;
+        if (threadIdx.x % LANES == 0) mine[wave * N + which] = v[0];
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            float s = mine[first * N + i];
-#pragma unroll
-            for (int k = 1; k < WAVES; ++k) s += mine[(first + k) * N + i];
-            v[i] = s;
-        }
+        v[0] = lanes_sum<WAVES>(mine[(first + threadIdx.x % WAVES) * N + which]);
+    }
+    if constexpr (HALVES) {
+        const auto r = swapped(v[0], v[0]);
+        v[0] = __uint_as_float(r[0]);
+        v[N - 1] = __uint_as_float(r[1]);
     }
 }
 
@@ -84,6 +95,24 @@ __device__ __forceinline__ float inverse_sqrt(float v)
 {
     const bool small = v < 0x1p-100f;
     return __builtin_amdgcn_rsqf(small ? v * 0x1p100f : v) * (small ? 0x1p50f : 1.f);
+}
+
+// t / n, rounded as the division is: one step from t times the rounded 1 / n.  (sum times 1 / n alone misses the mean of a constant
+// row by an ulp at every fourth width: 0.02 of the centred value 0 for rows of 1000 and an eps of 1e-5.)
+__device__ __forceinline__ float quotient(float t, float n, float inv_n)
+{
+    const float q = t * inv_n;
+    return __builtin_amdgcn_div_fixupf(fmaf(fmaf(-q, n, t), inv_n, q), n, t);  // (of infinities and NaN)
+}
+
+// What the centred values v = x - mu of a row still sum up to is the error of mu, an ulp or more of it where the sum was rounded:
+// their mean `off` goes with the squares' sum through one reduction, and what follows takes the mean as mu + off.  So a mean far
+// above the spread costs rounding of the inputs' differences alone.
+struct Statistics { float off, rstd; };
+__device__ __forceinline__ Statistics row_statistics(float squares, float sum, float inv_n, float eps)
+{
+    const float off = sum * inv_n, var = fmaf(-off, off, squares * inv_n);
+    return {off, inverse_sqrt((var < 0.f ? 0.f : var) + eps)};  // (under 0 by rounding alone; NaN stays)
 }
 
 // sum of f(k) g(k), k < N, in two chains of fma
@@ -243,44 +272,46 @@ __device__ __forceinline__ V kept(V v, bool keep)
     return v;
 }
 
-// N affine parameters from `col` on, fp32 or of the rows' type; `none` where there are none
-template <class T, int N>
+// N affine parameters from `col` on, fp32 or of the rows' type; `none` where there are none.  WHOLE: all N are in the row
+template <class T, bool WHOLE, int N>
 __device__ __forceinline__ void load_affine(const void *p, bool fp32, uint32_t col, uint32_t width, float none, float (&v)[N])
 {
 #pragma unroll
     for (int k = 0; k < N; ++k) v[k] = none;
     if (!p) return;
     if (fp32) {
-        if (col + N <= width) __builtin_memcpy(v, (const float *)p + col, sizeof(v));
+        if (WHOLE || col + N <= width) __builtin_memcpy(v, (const float *)p + col, sizeof(v));
         else
 #pragma unroll
             for (int k = 0; k < N; ++k)
                 if (col + k < width) v[k] = ((const float *)p)[col + k];
     } else {
-        const Vec<T, N> t = load_vec((const T *)p, col, width);
+        Vec<T, N> t;
+        if constexpr (WHOLE) __builtin_memcpy(&t, (const T *)p + col, sizeof(t));
+        else t = load_vec((const T *)p, col, width);
 #pragma unroll
         for (int k = 0; k < N; ++k) v[k] = (float)t.e[k];
     }
 }
 
 // ---- forward ---------------------------------------------------------------------------------------------------------------
-// Two sums over the row's registers (mean, then squares about it), one fma an element with weight and bias, which stay in
-// registers.  Bound by HBM: 2097152 x 64 fp16 in 94 us (5.7 TB/s), 8192 x 4096 bf16 in 24 us (5.6 TB/s).  Groups of more than
-// a wave load the next row while they work on one; smaller ones have enough waves without (2097152 x 64 fp16: 94 us without,
-// 101 us with).  16-bit rows of 256 threads and more are held to 64 registers, 8 waves: with the 66 that the compiler would take
-// a CU holds one workgroup of 1024 threads in place of two (6709 x 5001 bf16: 32 us, and 39 without).
+// Two reductions over the row's registers (mean; squares and what is left of the sum about it), two fma an element with weight
+// and bias, which stay in registers.  Bound by HBM: 2097152 x 64 fp16 in 94 us (5.7 TB/s), 8192 x 4096 bf16 in 24 us (5.6 TB/s).
+// Groups of more than a wave load the next row while they work on one; smaller ones have enough waves without (2097152 x 64 fp16:
+// 94 us without, 101 us with).  16-bit rows that leave lanes of their group idle are bound by the vector units beside (16376 x 2049
+// bf16 32 us, 6709 x 5001 32 us; with every lane's elements masked 40 and 42 us).
 template <class T, int G, int ITER, Access A>
-__global__ void __launch_bounds__(G > 256 ? G : 256, sizeof(T) == 2 && G >= 256 && ITER == 1 ? 8 : 1)
+__global__ void __launch_bounds__(G > 256 ? G : 256)
 k_ln_forward(const T *__restrict__ x, uint64_t xs, const void *__restrict__ w, const void *__restrict__ b, int affine_fp32,
              T *__restrict__ y, float *__restrict__ mean, float *__restrict__ rstd, uint64_t rows, uint32_t width,
              float inv_width, float eps)
 {
     constexpr int N = Vec16<T>::N, THREADS = G > 256 ? G : 256, GROUPS = THREADS / G;
-    __shared__ float lds[G > 64 ? 32 : 1];
+    __shared__ float lds[G > 64 ? 64 : 1];
     int turn = 0;
+    const float n = (float)width;
     const uint32_t lane = threadIdx.x % G, group = threadIdx.x / G;
     const uint64_t x_at = group * xs, y_at = (uint64_t)group * width;
-    const bool covered = width == (uint32_t)(G * N * ITER);
     Vec<T, N> raw[ITER];
     auto load_row = [&](uint64_t tile) {
         const Rows<T, A, GROUPS> from(x, xs, tile * GROUPS, group, x_at, rows, width);
@@ -292,14 +323,25 @@ k_ln_forward(const T *__restrict__ x, uint64_t xs, const void *__restrict__ w, c
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
         const Place p = place<N, A>(i * G + lane, width);
-        load_affine<T>(w, affine_fp32, p.at, width, 1.f, wv[i]);
-        load_affine<T>(b, affine_fp32, p.at, width, 0.f, bv[i]);
+        load_affine<T, A != TINY>(w, affine_fp32, p.at, width, 1.f, wv[i]);
+        load_affine<T, A != TINY>(b, affine_fp32, p.at, width, 0.f, bv[i]);
     }
-    // whether element k of vector i counts in the sums
-    auto counts = [&](int i, int k) {
+    // 1 where element k of vector i counts in the sums.  A group is the smallest that covers the row, so the first half of a lane's
+    // vectors is whole, and of the rest that of most waves above one a row: nothing is masked there.
+    constexpr int FIRST = ITER / 2;
+    float mask[ITER - FIRST][N];
+    bool all = true;
+#pragma unroll
+    for (int i = FIRST; i < ITER; ++i) {
         const Place p = place<N, A>(i * G + lane, width);
-        return k >= (int)p.twice && p.at + k < width;
-    };
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const bool counts = A == TINY ? p.at + k < width : k >= (int)p.twice;
+            mask[i - FIRST][k] = counts ? 1.f : 0.f;
+            all = all && counts;
+        }
+    }
+    const bool whole = __all(all);
     for (uint64_t tile = blockIdx.x; tile * GROUPS < rows; tile += gridDim.x) {
         const uint64_t row0 = tile * GROUPS;
         const int64_t left = mean ? (int64_t)(rows - row0) : 0;  // (of the statistics)
@@ -308,31 +350,40 @@ k_ln_forward(const T *__restrict__ x, uint64_t xs, const void *__restrict__ w, c
         for (int i = 0; i < ITER; ++i) {
 #pragma unroll
             for (int k = 0; k < N; ++k) v[i][k] = (float)raw[i].e[k];
-            if (covered) t[0] += pairwise<N>([&](int k) { return v[i][k]; });
-            else t[0] += pairwise<N>([&](int k) { return counts(i, k) ? v[i][k] : 0.f; });
+            if (i < FIRST || whole) t[0] += pairwise<N>([&](int k) { return v[i][k]; });
+            else t[0] += dot<N>([&](int k) { return v[i][k]; }, [&](int k) { return mask[i - FIRST][k]; });
         }
         if constexpr (G > 64) load_row(tile + gridDim.x);
         group_sum<G>(t, lds, turn);
-        const float mu = t[0] * inv_width;
-        t[0] = 0.f;
+        const float mu = quotient(t[0], n, inv_width);
+        float c[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
 #pragma unroll
             for (int k = 0; k < N; ++k) v[i][k] -= mu;
-            if (covered) t[0] += dot<N>([&](int k) { return v[i][k]; }, [&](int k) { return v[i][k]; });
-            else t[0] += dot<N>([&](int k) { return counts(i, k) ? v[i][k] : 0.f; }, [&](int k) { return v[i][k]; });
+            if (i < FIRST || whole) {
+                c[0] += dot<N>([&](int k) { return v[i][k]; }, [&](int k) { return v[i][k]; });
+                c[1] += pairwise<N>([&](int k) { return v[i][k]; });
+            } else {
+                float once[N];
+#pragma unroll
+                for (int k = 0; k < N; ++k) once[k] = v[i][k] * mask[i - FIRST][k];
+                c[0] += dot<N>([&](int k) { return once[k]; }, [&](int k) { return v[i][k]; });
+                c[1] += pairwise<N>([&](int k) { return once[k]; });
+            }
         }
-        group_sum<G>(t, lds, turn);
-        const float rs = inverse_sqrt(t[0] * inv_width + eps);
+        group_sum<G>(c, lds, turn);
+        const Statistics st = row_statistics(c[0], c[1], inv_width, eps);
+        const float rs = st.rstd, shift = -st.off * rs;
         const Rows<T, A, GROUPS> to(y, width, row0, group, y_at, rows, width);
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
             Vec<T, N> o;
 #pragma unroll
-            for (int k = 0; k < N; ++k) o.e[k] = (T)fmaf(v[i][k] * rs, wv[i][k], bv[i][k]);
+            for (int k = 0; k < N; ++k) o.e[k] = (T)fmaf(fmaf(v[i][k], rs, shift), wv[i][k], bv[i][k]);
             to.store(place<N, A>(i * G + lane, width), o);
         }
-        buffer_store(rows_buffer(mean + row0, left, 4, 4), lane == 0 ? group * 4 : OUTSIDE, mu);
+        buffer_store(rows_buffer(mean + row0, left, 4, 4), lane == 0 ? group * 4 : OUTSIDE, mu + st.off);
         buffer_store(rows_buffer(rstd + row0, left, 4, 4), lane == 0 ? group * 4 : OUTSIDE, rs);
         if constexpr (G <= 64) load_row(tile + gridDim.x);
     }
@@ -346,8 +397,9 @@ k_ln_forward_long(const T *__restrict__ x, uint64_t xs, const void *__restrict__
                   float inv_width, float eps)
 {
     constexpr int N = Vec16<T>::N;
-    __shared__ float lds[32];
+    __shared__ float lds[64];
     int turn = 0;
+    const float n = (float)width;
     for (uint64_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const T *xr = x + row * xs;
         float t[1] = {0.f};
@@ -356,24 +408,29 @@ k_ln_forward_long(const T *__restrict__ x, uint64_t xs, const void *__restrict__
             t[0] += pairwise<N>([&](int k) { return (float)v.e[k]; });
         }
         group_sum<1024>(t, lds, turn);
-        const float mu = t[0] * inv_width;
-        t[0] = 0.f;
+        const float mu = quotient(t[0], n, inv_width);
+        float s[2] = {0.f, 0.f};
         for (uint64_t c = threadIdx.x * N; c < width; c += 1024 * N) {
             const Vec<T, N> v = load_vec(xr, (uint32_t)c, width);
-            t[0] += pairwise<N>([&](int k) { const float d = c + k < width ? (float)v.e[k] - mu : 0.f; return d * d; });
+            float d[N];
+#pragma unroll
+            for (int k = 0; k < N; ++k) d[k] = c + k < width ? (float)v.e[k] - mu : 0.f;
+            s[0] += dot<N>([&](int k) { return d[k]; }, [&](int k) { return d[k]; });
+            s[1] += pairwise<N>([&](int k) { return d[k]; });
         }
-        group_sum<1024>(t, lds, turn);
-        const float rs = inverse_sqrt(t[0] * inv_width + eps);
+        group_sum<1024>(s, lds, turn);
+        const Statistics st = row_statistics(s[0], s[1], inv_width, eps);
+        const float rs = st.rstd, shift = -st.off * rs;
         for (uint64_t c = threadIdx.x * N; c < width; c += 1024 * N) {
             Vec<T, N> v = load_vec(xr, (uint32_t)c, width);
             float wv[N], bv[N];
-            load_affine<T>(w, affine_fp32, (uint32_t)c, width, 1.f, wv);
-            load_affine<T>(b, affine_fp32, (uint32_t)c, width, 0.f, bv);
+            load_affine<T, false>(w, affine_fp32, (uint32_t)c, width, 1.f, wv);
+            load_affine<T, false>(b, affine_fp32, (uint32_t)c, width, 0.f, bv);
 #pragma unroll
-            for (int k = 0; k < N; ++k) v.e[k] = (T)fmaf(((float)v.e[k] - mu) * rs, wv[k], bv[k]);
+            for (int k = 0; k < N; ++k) v.e[k] = (T)fmaf(fmaf((float)v.e[k] - mu, rs, shift), wv[k], bv[k]);
             store_vec(y + row * width, (uint32_t)c, width, v);
         }
-        if (mean && threadIdx.x == 0) { mean[row] = mu; rstd[row] = rs; }
+        if (mean && threadIdx.x == 0) { mean[row] = mu + st.off; rstd[row] = rs; }
     }
 }
 
@@ -442,7 +499,7 @@ k_ln_backward(const T *__restrict__ dy, uint64_t dys, const T *__restrict__ x, u
     float wv[HELD ? ITER : 1][N], sw[ITER][N], sb[ITER][N];
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
-        if constexpr (HELD) load_affine<T>(w, affine_fp32, place<N, A>(i * G + lane, width).at, width, 1.f, wv[i]);
+        if constexpr (HELD) load_affine<T, A != TINY>(w, affine_fp32, place<N, A>(i * G + lane, width).at, width, 1.f, wv[i]);
 #pragma unroll
         for (int k = 0; k < N; ++k) sw[i][k] = sb[i][k] = 0.f;
     }
@@ -465,7 +522,7 @@ k_ln_backward(const T *__restrict__ dy, uint64_t dys, const T *__restrict__ x, u
             if constexpr (!HELD) {
                 uint32_t at = place<N, A>(i * G + lane, width).at;
                 asm volatile("" : "+v"(at));  // (or the compiler takes the loads out of the loop, and spills)
-                load_affine<T>(w, affine_fp32, at, width, 1.f, wv[0]);
+                load_affine<T, A != TINY>(w, affine_fp32, at, width, 1.f, wv[0]);
             }
 #pragma unroll
             for (int k = 0; k < N; ++k) {
@@ -552,7 +609,7 @@ k_ln_backward_long_rows(const T *__restrict__ dy, uint64_t dys, const T *__restr
             for (uint64_t at = threadIdx.x * N; at < width; at += BWD_THREADS * N) {
                 const Vec<T, N> xv = load_vec(xr, (uint32_t)at, width), dv = load_vec(dr, (uint32_t)at, width);
                 float wv[N], h[N], g[N];
-                load_affine<T>(w, affine_fp32, (uint32_t)at, width, 1.f, wv);
+                load_affine<T, false>(w, affine_fp32, (uint32_t)at, width, 1.f, wv);
 #pragma unroll
                 for (int k = 0; k < N; ++k) { h[k] = ((float)xv.e[k] - mu) * rs; g[k] = (float)dv.e[k] * wv[k]; }
                 if (pass == 0) {
