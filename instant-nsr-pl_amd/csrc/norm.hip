@@ -439,13 +439,14 @@ constexpr int BWD_THREADS = 1024;
 
 template <class W> __device__ __forceinline__ void put_column(void *p, uint32_t col, float v) { ((W *)p)[col] = (W)v; }
 
-// sums of a workgroup's rows for its columns: one workgroup alone stores the results, of several each stores a row of partial
-// sums [2][width]
+// sums of a share of the rows for a column: of one share alone they are the results, of several each stores a row of partial sums
+// [2][width]
 template <class T>
-__device__ __forceinline__ void store_sum(int which, uint32_t col, float v, uint32_t width, float *part, void *dw, void *db, int affine_fp32)
+__device__ __forceinline__ void store_sum(uint32_t share, uint32_t shares, int which, uint32_t col, float v, uint32_t width, float *part,
+                                          void *dw, void *db, int affine_fp32)
 {
-    if (gridDim.x > 1) {
-        part[((uint64_t)blockIdx.x * 2 + which) * width + col] = v;
+    if (shares > 1) {
+        part[((uint64_t)share * 2 + which) * width + col] = v;
     } else if (void *p = which ? db : dw) {
         affine_fp32 ? put_column<float>(p, col, v) : put_column<T>(p, col, v);
     }
@@ -560,7 +561,8 @@ k_ln_backward(const T *__restrict__ dy, uint64_t dys, const T *__restrict__ x, u
     // the sum of element k of vector i of a lane is a column's where it counts
     auto put_sum = [&](int which, int i, uint32_t of_lane, int k, float v) {
         const Place p = place<N, A>(i * G + of_lane, width);
-        if (k >= (int)p.twice && p.at + k < width) store_sum<T>(which, p.at + k, v, width, part, dw, db, affine_fp32);
+        if (k >= (int)p.twice && p.at + k < width)
+            store_sum<T>(blockIdx.x, gridDim.x, which, p.at + k, v, width, part, dw, db, affine_fp32);
     };
 #pragma unroll
     for (int i = 0; i < ITER; ++i)
@@ -627,7 +629,8 @@ k_ln_backward_long_rows(const T *__restrict__ dy, uint64_t dys, const T *__restr
     }
 }
 
-// long rows: dw and db alone, a workgroup for 1024 N columns (blockIdx.y) of some of the rows (blockIdx.x)
+// long rows: dw and db alone, a workgroup for 1024 N columns (blockIdx.x: the axis that takes more than 65535) of a share of the rows
+// (blockIdx.y)
 template <class T>
 __global__ void __launch_bounds__(BWD_THREADS)
 k_ln_backward_long_columns(const T *__restrict__ dy, uint64_t dys, const T *__restrict__ x, uint64_t xs,
@@ -635,15 +638,15 @@ k_ln_backward_long_columns(const T *__restrict__ dy, uint64_t dys, const T *__re
                            void *db, int affine_fp32, uint64_t rows, uint32_t width)
 {
     constexpr int N = Vec16<T>::N;
-    const Place p = place<N, GLOBAL>(blockIdx.y * BWD_THREADS + threadIdx.x, width);
+    const Place p = place<N, GLOBAL>(blockIdx.x * BWD_THREADS + threadIdx.x, width);
     if (p.twice >= N) return;
     float sw[N] = {}, sb[N] = {};
-    for (uint64_t row0 = blockIdx.x; row0 < rows; row0 += 4ull * gridDim.x) {  // four rows under way
+    for (uint64_t row0 = blockIdx.y; row0 < rows; row0 += 4ull * gridDim.y) {  // four rows under way
         Vec<T, N> xv[4], dv[4];
         float mu[4], rs[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            const uint64_t r = row0 + (uint64_t)u * gridDim.x, row = r < rows ? r : rows - 1;
+            const uint64_t r = row0 + (uint64_t)u * gridDim.y, row = r < rows ? r : rows - 1;
             __builtin_memcpy(&xv[u], x + row * xs + p.at, sizeof(xv[u]));
             __builtin_memcpy(&dv[u], dy + row * dys + p.at, sizeof(dv[u]));
             mu[u] = mean[row];
@@ -651,7 +654,7 @@ k_ln_backward_long_columns(const T *__restrict__ dy, uint64_t dys, const T *__re
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            if (row0 + (uint64_t)u * gridDim.x >= rows) break;
+            if (row0 + (uint64_t)u * gridDim.y >= rows) break;
 #pragma unroll
             for (int k = 0; k < N; ++k) {
                 sw[k] = fmaf((float)dv[u].e[k], ((float)xv[u].e[k] - mu[u]) * rs[u], sw[k]);
@@ -662,32 +665,37 @@ k_ln_backward_long_columns(const T *__restrict__ dy, uint64_t dys, const T *__re
 #pragma unroll
     for (int k = 0; k < N; ++k)
         if (k >= (int)p.twice) {
-            store_sum<T>(0, p.at + k, sw[k], width, part, dw, db, affine_fp32);
-            store_sum<T>(1, p.at + k, sb[k], width, part, dw, db, affine_fp32);
+            store_sum<T>(blockIdx.y, gridDim.y, 0, p.at + k, sw[k], width, part, dw, db, affine_fp32);
+            store_sum<T>(blockIdx.y, gridDim.y, 1, p.at + k, sb[k], width, part, dw, db, affine_fp32);
         }
 }
 
-// the workgroups' partial sums [n][2 width] of 16 columns, 64 of them at a time; n = 0: no rows
+// the partial sums [n][2 width] of 16 columns at a time, 64 of them at once; n = 0: no rows
+constexpr uint32_t FINISH_MOST = 1u << 20;  // workgroups: a grid has less than 2^32 threads
 template <class T>
 __global__ void __launch_bounds__(1024)
 k_ln_backward_finish(const float *__restrict__ part, uint32_t n, uint32_t width, void *dw, void *db, int affine_fp32)
 {
-    const uint64_t col = (uint64_t)blockIdx.x * 16 + threadIdx.x % 16;
-    float acc = 0.f;
-    if (col < 2ull * width)
-#pragma unroll 8
-        for (uint32_t s = threadIdx.x / 16; s < n; s += 64) acc += part[s * 2ull * width + col];
-    acc += __shfl_xor(acc, 16, 64);
-    acc += __shfl_xor(acc, 32, 64);
     __shared__ float sums[16][16];
-    if ((threadIdx.x & 63) < 16) sums[threadIdx.x >> 6][threadIdx.x & 15] = acc;
-    __syncthreads();
-    if (threadIdx.x >= 16 || col >= 2ull * width) return;
-    float v = sums[0][threadIdx.x];
-    for (int q = 1; q < 16; ++q) v += sums[q][threadIdx.x];
-    void *p = col < width ? dw : db;
-    const uint32_t c = (uint32_t)(col < width ? col : col - width);
-    if (p) affine_fp32 ? put_column<float>(p, c, v) : put_column<T>(p, c, v);
+    for (uint64_t col0 = (uint64_t)blockIdx.x * 16; col0 < 2ull * width; col0 += (uint64_t)gridDim.x * 16) {
+        const uint64_t col = col0 + threadIdx.x % 16;
+        float acc = 0.f;
+        if (col < 2ull * width)
+#pragma unroll 8
+            for (uint32_t s = threadIdx.x / 16; s < n; s += 64) acc += part[s * 2ull * width + col];
+        acc += __shfl_xor(acc, 16, 64);
+        acc += __shfl_xor(acc, 32, 64);
+        if ((threadIdx.x & 63) < 16) sums[threadIdx.x >> 6][threadIdx.x & 15] = acc;
+        __syncthreads();
+        if (threadIdx.x < 16 && col < 2ull * width) {
+            float v = sums[0][threadIdx.x];
+            for (int q = 1; q < 16; ++q) v += sums[q][threadIdx.x];
+            void *p = col < width ? dw : db;
+            const uint32_t c = (uint32_t)(col < width ? col : col - width);
+            if (p) affine_fp32 ? put_column<float>(p, c, v) : put_column<T>(p, c, v);
+        }
+        __syncthreads();
+    }
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
@@ -873,13 +881,14 @@ extern "C" int nsr_layer_norm_backward(const void *dy, uint64_t dy_stride, const
                                    0, st, (const T *)dy, dy_stride, (const T *)x, x_stride, weight, fp32, mean, rstd, (T *)dx, rows,
                                    width, inv);
             if (affine)
-                hipLaunchKernelGGL((k_ln_backward_long_columns<T>), dim3(groups, nsr_div_up(width, BWD_THREADS * Vec16<T>::N)),
+                hipLaunchKernelGGL((k_ln_backward_long_columns<T>), dim3(nsr_div_up(width, BWD_THREADS * Vec16<T>::N), groups),
                                    dim3(BWD_THREADS), 0, st, (const T *)dy, dy_stride, (const T *)x, x_stride, mean, rstd,
                                    workspace, dweight, dbias, fp32, rows, width);
         }
+        const uint32_t columns = (uint32_t)nsr_div_up(2ull * width, 16);
         if (affine && groups != 1)
-            hipLaunchKernelGGL((k_ln_backward_finish<T>), dim3(nsr_div_up(2ull * width, 16)), dim3(1024), 0, st, workspace, groups,
-                               width, dweight, dbias, fp32);
+            hipLaunchKernelGGL((k_ln_backward_finish<T>), dim3(columns < FINISH_MOST ? columns : FINISH_MOST), dim3(1024), 0, st,
+                               workspace, groups, width, dweight, dbias, fp32);
         NSR_CHECK_LAUNCH("nsr_layer_norm_backward");
         return NSR_OK;
     });

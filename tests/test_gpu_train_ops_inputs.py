@@ -76,3 +76,31 @@ def test_layer_norm_forward_keeps_the_graph():
     assert all(torch.equal(p, q) for p, q in zip((y, mean, rstd), ops.layer_norm_forward(x, w, b)))
     with torch.no_grad():
         assert not ops.layer_norm_forward(x.clone().requires_grad_(), w, b)[0].requires_grad
+
+
+@pytest.mark.parametrize("rows,width", [(5, (1 << 25) + 3), (0, (1 << 25) + 3), (1, (1 << 28) + 4099), (6, (1 << 26) + 16)])
+def test_layer_norm_backward_of_very_wide_rows(rows, width):
+    """grids past 65535 blocks of columns, past 2^32 threads for the partial sums.  The products and the centred values are those of
+    torch's fp32 operations; sums of rows in another order, each of the rows additions off by u of the terms' sum at most.  dx is
+    looked at where one value of dy alone is not zero: its row's means are that term over the width."""
+    from nsr_hip import ops
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(rows, width, generator=g, device="cuda")
+    dy = torch.zeros_like(x)
+    mean, rstd = torch.full((rows,), 0.25, device="cuda"), torch.full((rows,), 1.5, device="cuda")
+    where = torch.tensor([0, 4095, 4096, width // 2 + 1, width - 4, width - 1], device="cuda")
+    for r in range(rows):
+        dy[r, where] = torch.randn(where.numel(), generator=g, device="cuda")
+    dx, dw, db = ops.layer_norm_backward(dy, x, None, mean, rstd)
+    assert dx.shape == x.shape and dw.shape == db.shape == (width,)
+    d, h = dy[:, where].double(), ((x[:, where] - 0.25) * 1.5).double()
+    bound = (rows + 2) * 2.0 ** -24
+    assert bool(((dw[where].double() - (d * h).sum(0)).abs() <= bound * (d * h).abs().sum(0)).all())
+    assert bool(((db[where].double() - d.sum(0)).abs() <= bound * d.abs().sum(0)).all())
+    assert int(torch.count_nonzero(dw)) <= where.numel() and int(torch.count_nonzero(db)) <= where.numel()
+    for r in range(rows):
+        a, c = float(d[r].sum()) / width, float((d[r] * h[r]).sum()) / width
+        want = 1.5 * (d[r] - a - h[r] * c)
+        assert bool(((dx[r, where].double() - want).abs() <= 16 * 2.0 ** -24 * (1.5 * d[r].abs() + want.abs() + 1e-6)).all())
+        rest = 1.5 * (-a - ((x[r, 7:4000:13] - 0.25) * 1.5).double() * c)
+        assert bool(((dx[r, 7:4000:13].double() - rest).abs() <= 64 * 2.0 ** -24 * (d[r].abs().sum() / width * 20)).all())
