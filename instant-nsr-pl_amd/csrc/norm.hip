@@ -766,19 +766,27 @@ Access access_of(uint32_t width, uint32_t dtype, const void *a, uint64_t as, con
                ? BUFFER : GLOBAL;
 }
 
-// workgroups of the backward pass = rows of partial sums
+// Shares of the rows in the backward pass, each with its row of partial sums.  Rows in registers: a workgroup a share, a CU a
+// workgroup.  Long rows: the columns' blocks are workgroups as well, so as many shares as give two a CU, and no more than 128 rows to
+// one.  (One row a share up to 256 of them took 2 GB of partial sums for 256 rows of 2^20 fp32, twice the input; now 16 MB.)
 uint32_t backward_groups(uint64_t rows, uint32_t width, uint32_t dtype)
 {
     if (rows == 0) return 0;
-    uint64_t per = 1;
-    if (width <= backward_most(dtype))
+    uint64_t per = 1, most = CUS;
+    if (width <= backward_most(dtype)) {
         ln_type(dtype, [&](auto t) {
             return row_shape<decltype(t), backward_most(sizeof(t) == 4 ? DT_F32 : DT_F16)>(width, [&](auto g, auto) {
                 per = BWD_THREADS / decltype(g)::value;
                 return 0;
             });
         });
-    const uint64_t tiles = (rows + per - 1) / per, most = CUS;
+    } else {
+        const uint64_t blocks = nsr_div_up(width, BWD_THREADS * (16 / dtype_size(dtype)));
+        const uint64_t few = (2 * CUS + blocks - 1) / blocks, deep = (rows + 127) / 128;
+        most = deep > few ? deep : few;
+        if (most > CUS) most = CUS;
+    }
+    const uint64_t tiles = (rows + per - 1) / per;
     // few rows: one workgroup does them all and needs no second launch (up to 4 tiles no slower alone, 12.9 instead of 16.8 us a
     // call in a row of calls; 8 tiles are slower alone)
     if (tiles <= 4) return 1;

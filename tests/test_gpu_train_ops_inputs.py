@@ -104,3 +104,21 @@ def test_layer_norm_backward_of_very_wide_rows(rows, width):
         assert bool(((dx[r, where].double() - want).abs() <= 16 * 2.0 ** -24 * (1.5 * d[r].abs() + want.abs() + 1e-6)).all())
         rest = 1.5 * (-a - ((x[r, 7:4000:13] - 0.25) * 1.5).double() * c)
         assert bool(((dx[r, 7:4000:13].double() - rest).abs() <= 64 * 2.0 ** -24 * (d[r].abs().sum() / width * 20)).all())
+
+
+@pytest.mark.parametrize("rows,width", [(5, 16385), (129, 40001), (300, 16386), (1100, 16385), (40, 1 << 20)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_column_sums_of_long_rows(rows, width, dtype):
+    """shares of several rows each: at most ceil(rows / shares) <= 128 additions a share and 128 over the shares, of terms with two
+    roundings of their own"""
+    from nsr_hip import ops
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x, dy = (torch.randn(rows, width, generator=g, device="cuda").to(dtype) for _ in range(2))
+    mean, rstd = (torch.rand(rows, generator=g, device="cuda") for _ in range(2))
+    _, dw, db = ops.layer_norm_backward(dy, x, None, mean, rstd, want_dx=False, affine_dtype=F32)
+    h = (x.double() - mean.double()[:, None]) * rstd.double()[:, None]
+    for got, terms in ((dw, dy.double() * h), (db, dy.double())):
+        bound = (128 + 128 + 4) * 2.0 ** -24 * (terms.abs().sum(0) if got is db
+                                                else (dy.double().abs() * (x.double().abs() + 1) * rstd.double()[:, None]).sum(0))
+        assert bool(((got.double() - terms.sum(0)).abs() <= bound).all())
+    assert all(torch.equal(p, q) for p, q in zip((dw, db), ops.layer_norm_backward(dy, x, None, mean, rstd, affine_dtype=F32)[1:]))

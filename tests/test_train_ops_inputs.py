@@ -71,3 +71,17 @@ def test_layer_norm_refuses_tangents(which):
         for call in calls:
             with pytest.raises(NsrError, match="forward mode"):
                 call()
+
+
+def test_partial_sums_of_long_rows_stay_small():
+    """the column sums' workspace of the backward pass, two fp32 rows a share of the rows: past the register form (more than 12288
+    columns of fp32, 16384 of 16 bits) a share has 128 rows, or fewer where two workgroups a CU need more shares"""
+    import nsr_hip
+    floats = nsr_hip.lib.nsr_layer_norm_backward_workspace_floats
+    for code, narrow, block in ((0, 12289, 4096), (1, 16385, 8192), (2, 16385, 8192)):
+        for width in (narrow, 20000, 65537, 1 << 20, (1 << 28) + 5, 1 << 30):
+            for rows in (0, 1, 4, 5, 64, 256, 1000, 5000, 1 << 20):
+                shares, left = divmod(floats(rows, width, code), 2 * width)
+                assert left == 0 and shares <= min(rows, 256)
+                assert shares <= max(-(-rows // 128), -(-512 // -(-width // block))), (rows, width)
+    assert 4 * floats(256, 1 << 20, 0) == 1 << 24
