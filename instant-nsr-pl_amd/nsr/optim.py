@@ -49,7 +49,8 @@ class AdamW(torch.optim.Optimizer):
     ``eps`` are the same for all groups, ``lr`` and ``weight_decay`` are the group's.  Tensors whose ``grad`` is None are left
     as they are; the step count is one for all tensors.  An element whose gradient is not finite keeps its value and moments.
     Works with ``torch.amp.GradScaler`` without a synchronisation of its own: gradients are unscaled in the pass, a step with a
-    non-finite one is left out.  32-bit state dicts can be exchanged with ``torch.optim.AdamW``'s."""
+    non-finite one is left out.  32-bit state dicts can be exchanged with ``torch.optim.AdamW``'s (which rounds the moments of
+    16-bit parameters to their type)."""
 
     _step_supports_amp_scaling = True
 
@@ -342,8 +343,8 @@ class AdamW(torch.optim.Optimizer):
         return sd
 
     def load_state_dict(self, state_dict):
-        """state of an optimizer with the same tensors and the same ``state_bits`` for each of them (the moments keep their own
-        types, unlike in torch, which casts them to the parameter's)"""
+        """state of an optimizer with the same tensors and the same ``state_bits`` for each of them.  32-bit moments stay float32,
+        also of 16-bit parameters, and take in those of 16 bits that ``torch.optim.AdamW`` keeps for them"""
         saved, steps = state_dict["state"], set()
         if any(g.get("amsgrad") or g.get("maximize") for g in state_dict["param_groups"]):
             raise NotImplementedError("AdamW: neither amsgrad nor maximize")
@@ -352,7 +353,8 @@ class AdamW(torch.optim.Optimizer):
                 continue
             for k, t in self.state[p].items():
                 v = saved[i].get(k)
-                if v is None or v.dtype != t.dtype or v.shape != t.shape:
+                if v is None or v.dtype not in ((F32, torch.float16, torch.bfloat16) if t.dtype is F32 else (t.dtype,)) or \
+                        v.shape != t.shape:
                     raise ValueError(f"AdamW.load_state_dict: tensor {i} needs {k} {tuple(t.shape)} {t.dtype}, the state has "
                                      f"{None if v is None else (tuple(v.shape), v.dtype)}")
             if "step" not in saved[i]:
