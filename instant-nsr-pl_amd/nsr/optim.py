@@ -34,7 +34,8 @@ class AdamW(torch.optim.Optimizer):
 
     ``max_grad_norm``: gradients are scaled by min(1, max_grad_norm / (norm + 1e-6)) with the norm over the gradients of all
     tensors; a step whose norm is not finite is left out whole.  ``grad_norm`` holds the last step's norm (a 0-dim GPU tensor that
-    the next step overwrites).  Nothing is read back to the host.
+    the next step overwrites).  Nothing is read back to the host.  ``max_grad_norm`` and ``capturable`` may be set later on; what a
+    captured step does stays as captured.
 
     ``capturable=True``: the step count lives on the device and ``step`` may be captured into a graph; the learning rate that a
     replay uses is a group's ``lr`` tensor (0-dim or one element, float32, on the GPU) or, if it is a number, the captured one.
@@ -58,27 +59,55 @@ class AdamW(torch.optim.Optimizer):
                  max_grad_norm=None, capturable=False, modules=(), rounding_seed=0):
         if state_bits not in (8, 32):
             raise ValueError(f"AdamW: state_bits is 8 or 32, got {state_bits}")
-        if max_grad_norm is not None and not 0.0 < float(max_grad_norm) < math.inf:
-            raise ValueError(f"AdamW: max_grad_norm {max_grad_norm}")
+        max_grad_norm = self._checked_norm(max_grad_norm)
         if not 0 <= int(rounding_seed) < 1 << 32:
             raise ValueError(f"AdamW: rounding_seed is a 32-bit number, got {rounding_seed}")
         self._built = False
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
-        self.state_bits, self.min_8bit_size = int(state_bits), int(min_8bit_size)
-        self.max_grad_norm = None if max_grad_norm is None else float(max_grad_norm)
-        self.capturable, self.rounding_seed = bool(capturable), int(rounding_seed)
+        self._state_bits, self._min_8bit_size, self.rounding_seed = int(state_bits), int(min_8bit_size), int(rounding_seed)
+        self._capturable, self._max_grad_norm = bool(capturable), None
         self._step, self._step_dev, self._hyper, self._partials = 0, None, None, None
         self._lay_out()
         self._images = self._image_modules(modules)
         self._shared_hyperparameters()
         for g in self.param_groups:
             self._learning_rate(g)
-        if self.capturable or self.max_grad_norm is not None:
-            self._device_step()
-        if self.max_grad_norm is not None:
-            room = lib.nsr_grad_squares_capacity(self._desc, len(self._ps))
-            self._partials = torch.empty(room, dtype=torch.float64, device=self.device)
+        self.capturable, self.max_grad_norm = capturable, max_grad_norm
         self._built = True
+
+    # ---- settings ------------------------------------------------------------------------------------------------------------
+    state_bits = property(lambda self: self._state_bits, doc="fixed at construction: the moments are laid out for it")
+    min_8bit_size = property(lambda self: self._min_8bit_size, doc="fixed at construction: the moments are laid out for it")
+
+    @property
+    def capturable(self):
+        return self._capturable
+
+    @capturable.setter
+    def capturable(self, value):
+        if value:
+            self._device_step()
+        self._capturable = bool(value)
+
+    @staticmethod
+    def _checked_norm(value):
+        if value is not None and not 0.0 < float(value) < math.inf:
+            raise ValueError(f"AdamW: max_grad_norm {value}")
+        return None if value is None else float(value)
+
+    @property
+    def max_grad_norm(self):
+        return self._max_grad_norm
+
+    @max_grad_norm.setter
+    def max_grad_norm(self, value):
+        value = self._checked_norm(value)
+        if value is not None:
+            self._device_step()
+            if self._partials is None:
+                room = lib.nsr_grad_squares_capacity(self._desc, len(self._ps))
+                self._partials = torch.empty(room, dtype=torch.float64, device=self.device)
+        self._max_grad_norm = value
 
     # ---- construction --------------------------------------------------------------------------------------------------------
     def _lay_out(self):
@@ -105,7 +134,7 @@ class AdamW(torch.optim.Optimizer):
         self._all_contiguous = all(p.is_contiguous() for p in self._ps)
         self._addresses = [p.data_ptr() for p in self._ps]
         self._kinds = [list(map(of, self._ps)) for of in (_size, _dtype, _device)]
-        self._bits = [8 if self.state_bits == 8 and p.numel() >= self.min_8bit_size else 32 for p in self._ps]
+        self._bits = [8 if self._state_bits == 8 and p.numel() >= self._min_8bit_size else 32 for p in self._ps]
         n = np.array([p.numel() for p in self._ps], dtype=np.int64)
         eight = np.array([b == 8 for b in self._bits])
         room = -(-n // BLOCK) * BLOCK
@@ -194,7 +223,7 @@ class AdamW(torch.optim.Optimizer):
         if isinstance(lr, torch.Tensor):
             if lr.numel() != 1 or lr.dtype != F32:
                 raise ValueError(f"AdamW: a learning rate tensor has one float32 element, got {tuple(lr.shape)} {lr.dtype}")
-            if self.capturable:
+            if self._capturable:
                 if lr.device != self.device:
                     raise ValueError(f"AdamW: the learning rate of a capturable optimizer is on {self.device}, got {lr.device}")
                 return 0.0, lr.data_ptr()
@@ -223,7 +252,7 @@ class AdamW(torch.optim.Optimizer):
     @property
     def grad_norm(self):
         """norm of the last step's gradients before clipping (None without ``max_grad_norm``)"""
-        return self._hyper[5] if self.max_grad_norm is not None else None
+        return self._hyper[5] if self._max_grad_norm is not None else None
 
     # ---- one step ------------------------------------------------------------------------------------------------------------
     def _gather(self):
@@ -290,7 +319,7 @@ class AdamW(torch.optim.Optimizer):
         scale, found = getattr(self, "grad_scale", None), getattr(self, "found_inf", None)
         if self._step_dev is None and (scale is not None or found is not None):
             self._device_step()  # (a step may be left out: only the device knows the count)
-        if not self.capturable and torch.cuda.is_current_stream_capturing():
+        if not self._capturable and torch.cuda.is_current_stream_capturing():
             raise NsrError("AdamW: only an optimizer with capturable=True can step inside a graph capture")
         f = self._fields
         rates = [self._learning_rate(g) for g in self.param_groups]
@@ -329,11 +358,11 @@ class AdamW(torch.optim.Optimizer):
         step, hyper = self._step_dev.data_ptr(), self._hyper.data_ptr()
         scale = None if scale is None else scale.data_ptr()
         found = None if found is None else found.data_ptr()
-        if self.max_grad_norm is None:
+        if self._max_grad_norm is None:
             check(lib.nsr_adamw_begin(step, hyper, b1, b2, None, 0, 0.0, scale, found, stream), "nsr_adamw_begin")
             return
         check(lib.nsr_adamw_begin_clipped(desc, n, self._partials.data_ptr(), self._partials.numel(), step, hyper, b1, b2,
-                                          self.max_grad_norm, scale, found, stream), "nsr_adamw_begin_clipped")
+                                          self._max_grad_norm, scale, found, stream), "nsr_adamw_begin_clipped")
 
     # ---- checkpoints ---------------------------------------------------------------------------------------------------------
     def state_dict(self):

@@ -44,3 +44,73 @@ def test_state_of_16_bit_parameters_is_exchanged_with_torch(dtype):
     eight = nsr.optim.AdamW(ps[1], state_bits=8, min_8bit_size=0, **kw)
     with pytest.raises(ValueError):
         eight.load_state_dict(theirs.state_dict())
+
+
+def _pair(n, seed=5):
+    import nsr.optim
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    p0 = torch.randn(n, generator=g, device="cuda")
+    gs = [torch.randn(n, generator=g, device="cuda") for _ in range(6)]
+    kw = dict(lr=0.01, betas=(0.9, 0.99), eps=1e-8)
+    return lambda **more: (lambda p: (p, nsr.optim.AdamW([p], **kw, **more)))(torch.nn.Parameter(p0.clone())), gs
+
+
+def test_clipping_switched_on_and_off_after_construction():
+    """the same bits as steps of optimizers built with each setting that hand their state on; a norm that is no norm is refused"""
+    new, gs = _pair(3000)
+    (p, opt), (q, plain), (r, clipped) = new(), new(), new(max_grad_norm=0.5)
+    assert opt.max_grad_norm is None and opt.grad_norm is None
+
+    def go(param, optimizer, g):
+        param.grad = g
+        optimizer.step()
+
+    def hand_on(a, b, of, to):
+        with torch.no_grad():
+            b.copy_(a)
+        to.load_state_dict(of.state_dict())
+
+    for g in gs[:2]:
+        go(p, opt, g), go(q, plain, g)
+    opt.max_grad_norm = 0.5
+    hand_on(q, r, plain, clipped)
+    for g in gs[2:4]:
+        go(p, opt, g), go(r, clipped, g)
+        assert torch.equal(opt.grad_norm, clipped.grad_norm) and abs(float(opt.grad_norm) / float(g.double().norm()) - 1) < 1e-6
+    assert torch.equal(p, r) and opt.taken_steps() == 4
+    opt.max_grad_norm = None
+    hand_on(r, q, clipped, plain)
+    for g in gs[4:]:
+        go(p, opt, g), go(q, plain, g)
+    # (the unclipped device-side step works 1 / (1 - b^t) out on the device, in 64 bits as on the host, rounded to fp32 once)
+    assert opt.grad_norm is None and opt.taken_steps() == 6 and torch.allclose(p, q, rtol=1e-6, atol=1e-8)
+    for bad in (0.0, -1.0, float("inf"), float("nan")):
+        with pytest.raises(ValueError):
+            opt.max_grad_norm = bad
+    assert opt.max_grad_norm is None
+    for name in ("state_bits", "min_8bit_size"):
+        with pytest.raises(AttributeError):
+            setattr(opt, name, 8)
+
+
+def test_capture_switched_on_after_construction():
+    """the count moves to the device: replays go on counting from where the eager steps stopped"""
+    new, gs = _pair(3000)
+    (p, opt), (q, ref) = new(), new(capturable=True)
+    held = torch.zeros_like(gs[0])
+    for g in gs[:2]:
+        p.grad = q.grad = g
+        opt.step(), ref.step()
+    opt.capturable = True
+    p.grad = held
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for g in gs[2:]:
+        held.copy_(g)
+        graph.replay()
+        q.grad = g
+        ref.step()
+        torch.cuda.synchronize()
+        assert torch.allclose(p, q, rtol=1e-6, atol=1e-8)
+    assert opt.taken_steps() == ref.taken_steps() == 6
