@@ -1050,7 +1050,8 @@ int nsr_masked_loss_backward(const float *pred, const float *target, const uint8
  * exp_avg_sq are e4m3 codes [n] of m and of sqrt(v), scales_m / scales_r float[ceil(n / 256)]: value = code * scale.  Codes are
  * rounded stochastically with bits from a hash of (seed, step, index0 + element); all-zero codes and scales are the zero state.
  * image (may be NULL): receives the fp16 image of the updated parameters.
- * An element whose (scaled) gradient is not finite keeps its parameter and moments. */
+ * An element whose (scaled) gradient is not finite keeps its parameter and moments (8-bit ones are rounded again with their block,
+ * under its new scale). */
 typedef struct NsrAdamwTensor {
     void *params;
     const void *grad;

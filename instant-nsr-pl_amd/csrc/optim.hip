@@ -5,7 +5,8 @@
 // Per element, g' = g * (unscale and clip factor):
 //   m' = b1 m + (1 - b1) g',   v' = b2 v + (1 - b2) g'^2,
 //   p' = p (1 - lr wd) - lr / (1 - b1^t) * m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
-// An element whose g' is not finite keeps p, m and v, as with every other AdamW kernel of the library.
+// An element whose g' is not finite keeps p, m and v, as with every other AdamW kernel of the library; 8-bit moments of it are
+// encoded again with their block, whose scale may be another now.
 //
 // 8-bit moments: blocks of 256 consecutive elements share one fp32 scale per moment; m and r = sqrt(v) are e4m3 codes,
 // scale = (largest magnitude of the block) / 448.  The root is held and not v because e4m3 spans 2^17.8: of r that is 2^35.6

@@ -48,7 +48,8 @@ class AdamW(torch.optim.Optimizer):
 
     Parameters are float32, float16 or bfloat16 (arithmetic and 32-bit moments in float32), dense and on one GPU; ``betas`` and
     ``eps`` are the same for all groups, ``lr`` and ``weight_decay`` are the group's.  Tensors whose ``grad`` is None are left
-    as they are; the step count is one for all tensors.  An element whose gradient is not finite keeps its value and moments.
+    as they are; the step count is one for all tensors.  An element whose gradient is not finite keeps its value and moments
+    (8-bit ones are rounded again with their block, under its new scale).
     Works with ``torch.amp.GradScaler`` without a synchronisation of its own: gradients are unscaled in the pass, a step with a
     non-finite one is left out.  32-bit state dicts can be exchanged with ``torch.optim.AdamW``'s (which rounds the moments of
     16-bit parameters to their type)."""

@@ -114,3 +114,38 @@ def test_capture_switched_on_after_construction():
         torch.cuda.synchronize()
         assert torch.allclose(p, q, rtol=1e-6, atol=1e-8)
     assert opt.taken_steps() == ref.taken_steps() == 6
+
+
+@pytest.mark.parametrize("size", [1024, 700])
+def test_8_bit_moments_beside_a_gradient_that_is_not_finite(size):
+    """the parameter stays; the moments are those of before, rounded once more: within one lattice step of the block's new scale
+    (steps of e4m3 value y: 2^(max(floor(log2 y), -6) - 3); a code may be rounded up to the next power's), signs kept, and
+    positive roots above zero"""
+    import nsr.optim
+    g = torch.Generator(device="cuda").manual_seed(8)
+    p = torch.nn.Parameter(torch.randn(size, generator=g, device="cuda"))
+    opt = nsr.optim.AdamW([p], lr=0.01, state_bits=8, min_8bit_size=0)
+    for _ in range(3):
+        p.grad = torch.randn(size, generator=g, device="cuda")
+        opt.step()
+
+    def moments():
+        s = opt.state[p]
+        per = s["scales"].double().repeat_interleave(256, dim=1)[:, :size]
+        return [s[k].double() * sc for k, sc in zip(("exp_avg", "exp_avg_rms"), per)], per
+
+    bad = torch.tensor([0, 5, 255, 300, 511, 600, size - 1], device="cuda")
+    for scale in (1.0, 100.0, 0.0):  # the blocks' scales stay about as they are, grow, shrink
+        before, _ = moments()
+        p0 = p.detach().clone()
+        p.grad = scale * torch.randn(size, generator=g, device="cuda")
+        p.grad[bad] = torch.tensor([float("nan"), float("inf"), -float("inf")], device="cuda").repeat(3)[:bad.numel()]
+        opt.step()
+        assert torch.equal(p[bad], p0[bad])
+        after, per = moments()
+        for a, b, sc in zip(after, before, per):
+            a, b, sc = a[bad], b[bad], sc[bad]
+            y = (b / sc).abs().clamp_min(2.0 ** -9)
+            step = torch.exp2(torch.floor(torch.log2(y)).clamp_min(-6) - 3) * sc
+            assert bool(((a - b).abs() <= step * (1 + 2.0 ** -20)).all()) and bool((a * b >= 0).all())
+        assert bool((after[1][bad] > 0).all())
