@@ -41,7 +41,8 @@ class AdamW(torch.optim.Optimizer):
     replay uses is a group's ``lr`` tensor (0-dim or one element, float32, on the GPU) or, if it is a number, the captured one.
 
     ``modules``: ``tinycudann`` modules whose ``params`` are among the parameters: the fp16 image that their kernels read is
-    written in the same pass (otherwise they cast ``params`` again in every forward pass).
+    written in the same pass (otherwise they cast ``params`` again in every forward pass).  ``refresh_images``: for parameters that
+    were written from outside between replays of a captured forward pass.
 
     ``flat32`` / ``flat8``: the moments of all tensors as one buffer each (``state`` holds views of them); ``set_step`` and
     ``taken_steps``: the step count.
@@ -320,7 +321,8 @@ class AdamW(torch.optim.Optimizer):
         scale, found = getattr(self, "grad_scale", None), getattr(self, "found_inf", None)
         if self._step_dev is None and (scale is not None or found is not None):
             self._device_step()  # (a step may be left out: only the device knows the count)
-        if not self._capturable and torch.cuda.is_current_stream_capturing():
+        capturing = torch.cuda.is_current_stream_capturing()
+        if capturing and not self._capturable:
             raise NsrError("AdamW: only an optimizer with capturable=True can step inside a graph capture")
         f = self._fields
         rates = [self._learning_rate(g) for g in self.param_groups]
@@ -350,7 +352,17 @@ class AdamW(torch.optim.Optimizer):
         torch.autograd.graph.increment_version(live)
         for m, i, image in self._images:
             m.adopt_shadow(image)
+            m._replayed = m._replayed or capturing
         return loss
+
+    def refresh_images(self):
+        """writes the ``modules``' fp16 images from their parameters.  An eager forward pass sees by itself that parameters were
+        written from outside; a captured one reads the image that the last step left, so call this between such a write and the next
+        replay (or take one eager step)"""
+        with torch.no_grad():
+            for m, i, image in self._images:
+                image.copy_(m.params)
+                m.adopt_shadow(image)
 
     def _begin(self, desc, n, b1, b2, scale, found, stream):
         for t in (scale, found):

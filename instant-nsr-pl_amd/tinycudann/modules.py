@@ -100,6 +100,8 @@ def _mlp_desc_from_config(n_in, n_out, cfg):
 class Module(torch.nn.Module):
     """One flat fp32 parameter + a lazily refreshed fp16 shadow that the kernels read."""
 
+    _replayed = False  # a captured optimizer step writes ``params``: replays of it bump no version counter
+
     def __init__(self, seed=1337):
         super().__init__()
         self.seed = seed
@@ -122,7 +124,7 @@ class Module(torch.nn.Module):
         # holds -- one 75 MB cast per chunk otherwise; a `.data` write in between needs invalidate().  NOT in train() mode, not
         # even under no_grad: the reference's sphere_init writes `.data` right after construction, possibly behind a forward
         # (tests/test_gpu_shims.py::test_sphere_init_through_params_data_is_seen_and_trains)
-        lazy_ok = not self.training
+        lazy_ok = not self.training and not self._replayed
         if self._shadow is None or key != self._shadow_key or not (self._shadow_trusted or (lazy_ok and self._shadow_lazy)):
             self._shadow = params.detach().to(torch.float16).contiguous()
             self._shadow_key, self._shadow_trusted, self._shadow_lazy = key, False, lazy_ok

@@ -149,3 +149,59 @@ def test_8_bit_moments_beside_a_gradient_that_is_not_finite(size):
             step = torch.exp2(torch.floor(torch.log2(y)).clamp_min(-6) - 3) * sc
             assert bool(((a - b).abs() <= step * (1 + 2.0 ** -20)).all()) and bool((a * b >= 0).all())
         assert bool((after[1][bad] > 0).all())
+
+
+def _module_and_graph(seed=3):
+    """a network whose optimizer's step is captured, its gradients in a buffer of their own"""
+    import nsr.optim
+    import tinycudann as tcnn
+    from conftest import COLOR_MLP
+    torch.manual_seed(seed)
+    net = tcnn.Network(16, 3, COLOR_MLP).cuda()
+    opt = nsr.optim.AdamW([net.params], lr=0.05, capturable=True, modules=[net])
+    net.params.grad = torch.randn_like(net.params)
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    return net, opt, graph
+
+
+def test_replayed_steps_and_parameters_written_from_outside():
+    """a replay bumps no version counter: a cast that evaluation mode made after a write from outside is not taken for the
+    parameters that a replay has changed since"""
+    net, opt, graph = _module_and_graph()
+    image = lambda: net.half_params(net.params)  # noqa: E731
+    now = lambda: net.params.detach().half()  # noqa: E731
+    for mode in (net.train, net.eval):
+        mode()
+        graph.replay()
+        assert torch.equal(image(), now())
+    with torch.no_grad():
+        net.params.add_(0.25)
+    for mode in (net.eval, net.train, net.eval):
+        mode()
+        assert torch.equal(image(), now())
+        graph.replay()
+        assert torch.equal(image(), now())
+    opt.step()  # an eager step puts the image right
+    graph.replay()
+    assert torch.equal(image(), now()) and net._shadow_trusted
+
+
+def test_captured_forward_reads_the_refreshed_image():
+    net, opt, graph = _module_and_graph()
+    x = torch.rand(256, 16, device="cuda")
+    with torch.no_grad():
+        net(x)
+        forward = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(forward):
+            y = net(x)
+        for k in range(3):
+            graph.replay()
+            forward.replay()
+            assert torch.equal(y, net(x))
+            net.params.mul_(0.5 + k)
+            opt.refresh_images()
+            forward.replay()
+            assert torch.equal(y, net(x)) and torch.equal(net.half_params(net.params), net.params.half())
