@@ -3,13 +3,13 @@
 set -e
 HERE="$(cd "$(dirname "$0")" && pwd)"
 OUT="${1:-$HERE/../nsr_hip}"
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -munsafe-fp-atomics -Wall -Wno-unused-function -Xclang -target-feature -Xclang -packed-fp32-ops ${NSR_EXTRA_FLAGS}"
+. "$HERE/flags.sh"
 mkdir -p "$HERE/obj"
 pids=()
-for f in util hashgrid gridmlp mlp vmlp neus march render fused occupancy step optim norm; do
-  ( hipcc $FLAGS -c "$HERE/$f.hip" -o "$HERE/obj/$f.o" ) &
+for f in $NSR_UNITS; do
+  ( hipcc $NSR_FLAGS ${NSR_EXTRA_FLAGS} -c "$HERE/$f.hip" -o "$HERE/obj/$f.o" ) &
   pids+=($!)
 done
 for p in "${pids[@]}"; do wait $p; done
-hipcc --offload-arch=gfx950 -shared -fPIC -o "$OUT/libnsr_hip.so" "$HERE"/obj/{util,hashgrid,gridmlp,mlp,vmlp,neus,march,render,fused,occupancy,step,optim,norm}.o
+hipcc --offload-arch=gfx950 -shared -fPIC -o "$OUT/libnsr_hip.so" $(nsr_objects "$HERE/obj")
 echo "built $OUT/libnsr_hip.so"

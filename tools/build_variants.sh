@@ -6,13 +6,13 @@ set -e
 HERE="$(cd "$(dirname "$0")/.." && pwd)"
 CS="$HERE/instant-nsr-pl_amd/csrc"
 OUT="$HERE/build/variants"; mkdir -p "$OUT"
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -munsafe-fp-atomics -Wall -Wno-unused-function"
+. "$CS/flags.sh"
 pids=()
 for spec in "$@"; do
   name="${spec%%:*}"; defs="${spec#*:}"
-  ( hipcc $FLAGS $defs -c "$CS/hashgrid.hip" -o "$OUT/hashgrid_$name.o" &&
+  ( hipcc $NSR_FLAGS $defs -c "$CS/hashgrid.hip" -o "$OUT/hashgrid_$name.o" &&
     hipcc --offload-arch=gfx950 -shared -fPIC -o "$OUT/libnsr_hip_$name.so" "$OUT/hashgrid_$name.o" \
-      "$CS"/obj/{util,gridmlp,mlp,vmlp,neus,march,render,fused,occupancy,step}.o && echo "built $name ($defs)" ) &
+      $(nsr_objects "$CS/obj" hashgrid) && echo "built $name ($defs)" ) &
   pids+=($!)
 done
 for p in "${pids[@]}"; do wait $p; done

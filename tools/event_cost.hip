@@ -1,7 +1,7 @@
 // What an event on a stream's chain costs on gfx950 / ROCm 7: a chain of short kernels on stream A with, between two of
 // them, (0) nothing, (1) hipEventRecord, (2) the event riding on the previous launch (hipExtLaunchKernelGGL stopEvent),
 // each with a second stream waiting on the event and launching a kernel of its own; (3) a hipStreamWaitEvent on A for an
-// event of stream B.   hipcc --offload-arch=gfx950 -O2 tools/event_cost.hip -o build/tmp/event_cost && build/tmp/event_cost
+// event of stream B.   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O2 tools/event_cost.hip -o build/tmp/event_cost && build/tmp/event_cost
 #include <hip/hip_runtime.h>
 #include <hip/hip_ext.h>
 #include <chrono>

@@ -8,7 +8,7 @@
 //   helper1:            wait F, Kbin (record J) ...... wait E, K3 ........ (record JW)
 //   helper2:                                            wait E, K4 -> helper1 waits for it
 //
-//   hipcc --offload-arch=gfx950 -O2 tools/fork_bubble.hip -o build/tmp/fork_bubble && build/tmp/fork_bubble
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O2 tools/fork_bubble.hip -o build/tmp/fork_bubble && build/tmp/fork_bubble
 #include <hip/hip_runtime.h>
 #include <hip/hip_ext.h>
 #include <algorithm>

@@ -1,5 +1,5 @@
 // Host cost of hipLaunchKernelGGL on gfx950 / ROCm 7 by kernel-argument size and dynamic LDS: an empty kernel launched 20,000
-// times back to back (the GPU keeps up), host time per launch.   hipcc --offload-arch=gfx950 -O2 tools/launch_cost.hip -o build/tmp/launch_cost
+// times back to back (the GPU keeps up), host time per launch.   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O2 tools/launch_cost.hip -o build/tmp/launch_cost
 #include <hip/hip_runtime.h>
 #include <chrono>
 #include <cstdio>

@@ -1,5 +1,5 @@
 // Microbenchmark: LDS atomic throughput on gfx950 (lane-ops per clock per CU) for the op types a gradient
-// accumulator could use.  Build: hipcc --offload-arch=gfx950 -O3 -munsafe-fp-atomics -o /tmp/ldsb tools/lds_atomics_bench.hip
+// accumulator could use.  Build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -munsafe-fp-atomics -o /tmp/ldsb tools/lds_atomics_bench.hip
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <stdio.h>

@@ -1,6 +1,6 @@
 // Does an event that rides on a launch (hipExtLaunchKernelGGL stopEvent) order a kernel on ANOTHER stream behind the launch's
 // COMPLETION?  Stream A: a kernel that spins ~20 us and then writes slot i; stream B waits for the event and checks the slot.
-//   hipcc --offload-arch=gfx950 -O2 tools/stop_event_order.hip -o build/tmp/stop_event_order && build/tmp/stop_event_order
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O2 tools/stop_event_order.hip -o build/tmp/stop_event_order && build/tmp/stop_event_order
 #include <hip/hip_runtime.h>
 #include <hip/hip_ext.h>
 #include <cstdio>
