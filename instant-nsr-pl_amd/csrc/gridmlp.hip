@@ -80,8 +80,9 @@ k_grid_mlp_forward(const float *__restrict__ x, const __half *__restrict__ table
 #pragma unroll
             for (int f = 0; f < F; ++f) {
                 const int c = 8 * g + i * F + f;
+                const float y = nsr_rounded(v[f]);  // (the plain encode's fp16 value)
                 // (columns [n_in, in_pad) of the MLP input are the constant 1, as in load_x8)
-                b[i * F + f] = c < (int)n_in ? (_Float16)__half2float(__float2half_rn(v[f])) : (_Float16)1;
+                b[i * F + f] = c < (int)n_in ? (_Float16)y : (_Float16)1;
             }
         }
         if (!valid) {

@@ -144,11 +144,11 @@ k_grid_forward(const float *__restrict__ x, const __half *__restrict__ table, __
         for (int q = 0; q < F * 3; ++q) jo[q] = 0.f;
     }
     if constexpr (F == 1) {
-        yo[0] = __float2half_rn(acc[0]);
+        yo[0] = nsr_half_of(acc[0]);
     } else {
 #pragma unroll
         for (int f = 0; f < F; f += 2)
-            *reinterpret_cast<__half2 *>(yo + f) = __floats2half2_rn(acc[f], acc[f + 1]);
+            *reinterpret_cast<__half2 *>(yo + f) = nsr_half2_of(acc[f], acc[f + 1]);
     }
 }
 
@@ -164,10 +164,10 @@ template <int F>
 __device__ __forceinline__ void store_enc(__half *yo, const float (&acc)[F])
 {
     if constexpr (F == 1) {
-        yo[0] = __float2half_rn(acc[0]);
+        yo[0] = nsr_half_of(acc[0]);
     } else {
 #pragma unroll
-        for (int f = 0; f < F; f += 2) *reinterpret_cast<__half2 *>(yo + f) = __floats2half2_rn(acc[f], acc[f + 1]);
+        for (int f = 0; f < F; f += 2) *reinterpret_cast<__half2 *>(yo + f) = nsr_half2_of(acc[f], acc[f + 1]);
     }
 }
 
@@ -286,11 +286,11 @@ __device__ __forceinline__ void blend8(const Cell &c, const float (&v)[8][F], __
         for (int f = 0; f < F; ++f) acc[f] = fmaf(w, v[k][f], acc[f]);
     }
     if constexpr (F == 1) {
-        yo[0] = __float2half_rn(acc[0]);
+        yo[0] = nsr_half_of(acc[0]);
     } else {
 #pragma unroll
         for (int f = 0; f < F; f += 2)  // (the same bits as the plain encode: fp32 sum, then fp16)
-            *reinterpret_cast<__half2 *>(yo + f) = __floats2half2_rn(nsr_rounded(acc[f]), nsr_rounded(acc[f + 1]));
+            *reinterpret_cast<__half2 *>(yo + f) = nsr_half2_of(acc[f], acc[f + 1]);
     }
 }
 

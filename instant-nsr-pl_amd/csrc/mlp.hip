@@ -275,7 +275,7 @@ k_mlp_dgrad(const void *__restrict__ dout, int dout_f32, uint32_t dout_stride, c
                         const float o = __half2float(out[(uint64_t)s * 16 + c]);
                         v *= o * (1.f - o);
                     }
-                    d_o[r] = v * grad_scale;
+                    d_o[r] = nsr_rounded(v * grad_scale);
                 }
             }
             if (gout) {  // column-blocked, 16 columns
@@ -445,7 +445,7 @@ k_mlp_dgrad_pair(const float *__restrict__ d_rgb /* [n,3] */, const float *__res
                     float v = d_rgb[(uint64_t)s * 3 + c];
                     const float o = __half2float(out_c[(uint64_t)s * 16 + c]);
                     v *= o * (1.f - o);
-                    d_o[r] = v * grad_scale;
+                    d_o[r] = nsr_rounded(v * grad_scale);
                 }
             }
 #pragma unroll
@@ -499,9 +499,9 @@ k_mlp_dgrad_pair(const float *__restrict__ d_rgb /* [n,3] */, const float *__res
         if (valid) {
             if (g == 0) dfeat[0] += d_logit[s];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) d_o[r] = dfeat[r] * grad_scale;
+            for (int r = 0; r < 4; ++r) d_o[r] = nsr_rounded(dfeat[r] * grad_scale);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) gout_d[t32_off(s, 4 * g + r, 16)] = __float2half_rn(nsr_rounded(d_o[r]));
+            for (int r = 0; r < 4; ++r) gout_d[t32_off(s, 4 * g + r, 16)] = __float2half_rn(d_o[r]);
         } else {
             d_o = f32x4{0.f, 0.f, 0.f, 0.f};
         }

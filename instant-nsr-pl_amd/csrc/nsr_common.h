@@ -73,6 +73,9 @@ __device__ __forceinline__ float nsr_rounded(float v)
     asm("" : "+v"(v));
     return v;
 }
+// fp32 sum or product, then fp16: for values that several kernels store and that are to be the same in all of them
+__device__ __forceinline__ __half nsr_half_of(float v) { return __float2half_rn(nsr_rounded(v)); }
+__device__ __forceinline__ __half2 nsr_half2_of(float a, float b) { return __floats2half2_rn(nsr_rounded(a), nsr_rounded(b)); }
 
 // fp32 -> bf16, round to nearest even (NaN stays NaN); two values packed low | high << 16
 __device__ __forceinline__ uint32_t nsr_to_bf16(float f)
