@@ -1,6 +1,7 @@
 """AdamW over any number of tensors for a user's own training system (the reference's ``parse_optimizer`` builds
 ``torch.optim.AdamW``: systems/utils.py:314-325; the trainers of this package own their optimizers and do not need it)."""
 import math
+from collections import defaultdict
 
 import numpy as np
 import torch
@@ -380,13 +381,25 @@ class AdamW(torch.optim.Optimizer):
     # ---- checkpoints ---------------------------------------------------------------------------------------------------------
     def state_dict(self):
         """torch's layout; every tensor's state holds the common ``step`` as well"""
-        sd, step = super().state_dict(), float(self.taken_steps())
-        sd["state"] = {k: {"step": torch.tensor(step), **v} for k, v in sd["state"].items()}
-        return sd
+        held, step = self.state, float(self.taken_steps())
+        self.state = defaultdict(dict, {p: {"step": torch.tensor(step), **s} for p, s in held.items()})
+        try:
+            return super().state_dict()  # (its hooks see the whole)
+        finally:
+            self.state = held
 
     def load_state_dict(self, state_dict):
         """state of an optimizer with the same tensors and the same ``state_bits`` for each of them.  32-bit moments stay float32,
         also of 16-bit parameters, and take in those of 16 bits that ``torch.optim.AdamW`` keeps for them"""
+        before, after = self._optimizer_load_state_dict_pre_hooks, self._optimizer_load_state_dict_post_hooks
+        state_dict = state_dict.copy()
+        for hook in before.values():
+            state_dict = hook(self, state_dict) or state_dict
+        self._load(state_dict)
+        for hook in after.values():
+            hook(self)
+
+    def _load(self, state_dict):
         saved, steps = state_dict["state"], set()
         if any(g.get("amsgrad") or g.get("maximize") for g in state_dict["param_groups"]):
             raise NotImplementedError("AdamW: neither amsgrad nor maximize")
@@ -405,7 +418,12 @@ class AdamW(torch.optim.Optimizer):
         if len(steps) > 1:
             raise ValueError(f"AdamW.load_state_dict: the tensors' step counts differ: {sorted(steps)}")
         rates = [g["lr"] for g in self.param_groups]
-        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
+        hooks = self._optimizer_load_state_dict_pre_hooks, self._optimizer_load_state_dict_post_hooks
+        self._optimizer_load_state_dict_pre_hooks, self._optimizer_load_state_dict_post_hooks = {}, {}
+        try:  # the groups alone: torch would cast the moments to the parameters' types
+            super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
+        finally:
+            self._optimizer_load_state_dict_pre_hooks, self._optimizer_load_state_dict_post_hooks = hooks
         for g, lr in zip(self.param_groups, rates):
             if isinstance(lr, torch.Tensor):  # (a captured step reads this tensor: it keeps its place)
                 lr.fill_(float(g["lr"]))

@@ -205,3 +205,29 @@ def test_captured_forward_reads_the_refreshed_image():
             opt.refresh_images()
             forward.replay()
             assert torch.equal(y, net(x)) and torch.equal(net.half_params(net.params), net.params.half())
+
+
+def test_state_dict_hooks_see_the_whole_state():
+    """as in torch: a hook behind state_dict sees the steps and may change them, one in front of load_state_dict gets and may replace
+    the moments, one behind it sees them loaded"""
+    new, gs = _pair(300)
+    (p, opt), (q, other) = new(), new()
+    p.grad = gs[0]
+    opt.step()
+    seen = []
+    opt.register_state_dict_post_hook(lambda o, sd: seen.append(sd["state"][0]["step"].item()))
+    sd = opt.state_dict()
+    assert seen == [1.0] and set(opt.state[p]) == {"exp_avg", "exp_avg_sq"} and list(sd["state"][0])[0] == "step"
+
+    def double(o, sd):
+        state = {0: {**sd["state"][0], "exp_avg": 2 * sd["state"][0]["exp_avg"]}}
+        return {**sd, "state": state}
+
+    first = other.register_load_state_dict_pre_hook(double)
+    second = other.register_load_state_dict_post_hook(lambda o: seen.append((o.state[q]["exp_avg"].clone(), o.taken_steps())))
+    other.load_state_dict(sd)
+    assert torch.equal(seen[1][0], 2 * opt.state[p]["exp_avg"]) and seen[1][1] == 1
+    assert torch.equal(other.state[q]["exp_avg_sq"], opt.state[p]["exp_avg_sq"])
+    first.remove(), second.remove()
+    other.load_state_dict(sd)
+    assert torch.equal(other.state[q]["exp_avg"], opt.state[p]["exp_avg"]) and len(seen) == 2
