@@ -185,16 +185,17 @@ class AdamW(torch.optim.Optimizer):
 
     def _image_modules(self, modules):
         place = {id(p): i for i, p in enumerate(self._ps)}
-        found = []
+        found, images = [], {}  # (modules of one parameter share its image)
         for m in modules:
             if m.params.numel() == 0:
                 continue
             i = place.get(id(m.params))
             if i is None or m.params.dtype != F32:
                 raise ValueError("AdamW: `modules` are tinycudann modules whose float32 `params` are among the parameters")
-            image = torch.empty_like(m.params, dtype=torch.float16)
-            self._desc[i].image = image.data_ptr()
-            found.append((m, i, image))
+            if i not in images:
+                images[i] = torch.empty_like(m.params, dtype=torch.float16)
+                self._desc[i].image = images[i].data_ptr()
+            found.append((m, i, images[i]))
         return found
 
     def add_param_group(self, param_group):

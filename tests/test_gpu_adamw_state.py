@@ -231,3 +231,19 @@ def test_state_dict_hooks_see_the_whole_state():
     first.remove(), second.remove()
     other.load_state_dict(sd)
     assert torch.equal(other.state[q]["exp_avg"], opt.state[p]["exp_avg"]) and len(seen) == 2
+
+
+def test_two_modules_of_one_parameter():
+    """the pass writes one image a parameter: both modules read it, in every step"""
+    import nsr.optim
+    import tinycudann as tcnn
+    from conftest import COLOR_MLP
+    torch.manual_seed(4)
+    a, b = (tcnn.Network(16, 3, COLOR_MLP).cuda() for _ in range(2))
+    b.params = a.params
+    opt = nsr.optim.AdamW([a.params], lr=0.05, modules=[a, b])
+    for _ in range(4):
+        a.params.grad = torch.randn_like(a.params)
+        opt.step()
+        for m in (a, b):
+            assert m._shadow_trusted and torch.equal(m.half_params(m.params), a.params.detach().half())
