@@ -198,6 +198,11 @@ class AdamW(torch.optim.Optimizer):
             found.append((m, i, images[i]))
         return found
 
+    def _image_owner(self, module, i):
+        if module.params is not self._ps[i]:
+            raise NsrError("AdamW: a module of `modules` has another `params` than at construction")
+        return module.params
+
     def add_param_group(self, param_group):
         if getattr(self, "_built", False):
             raise NotImplementedError("AdamW: the parameters are fixed at construction (their moments lie in flat buffers)")
@@ -340,7 +345,7 @@ class AdamW(torch.optim.Optimizer):
             return loss
         with device_guard(self.device), timed("adamw_step", n):
             for m, i, image in self._images:
-                p = m.params
+                p = self._image_owner(m, i)
                 if m._shadow is not image or not m._shadow_trusted or m._shadow_key != (p.data_ptr(), p._version, p.device):
                     image.copy_(p.detach())  # first step, or the parameters were written from outside
             s = stream_ptr()
@@ -363,7 +368,7 @@ class AdamW(torch.optim.Optimizer):
         replay (or take one eager step)"""
         with torch.no_grad():
             for m, i, image in self._images:
-                image.copy_(m.params)
+                image.copy_(self._image_owner(m, i))
                 m.adopt_shadow(image)
 
     def _begin(self, desc, n, b1, b2, scale, found, stream):

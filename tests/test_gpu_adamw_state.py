@@ -247,3 +247,23 @@ def test_two_modules_of_one_parameter():
         opt.step()
         for m in (a, b):
             assert m._shadow_trusted and torch.equal(m.half_params(m.params), a.params.detach().half())
+
+
+def test_a_module_with_another_parameter_is_refused():
+    """an image of the optimizer's parameter is not handed to a module that holds another one meanwhile"""
+    import nsr.optim
+    import tinycudann as tcnn
+    from conftest import COLOR_MLP
+    from nsr_hip import NsrError
+    net = tcnn.Network(16, 3, COLOR_MLP).cuda()
+    p = net.params
+    opt = nsr.optim.AdamW([p], lr=0.05, modules=[net])
+    p.grad = torch.ones_like(p)
+    opt.step()
+    before = p.detach().clone()
+    net.params = torch.nn.Parameter(torch.randn_like(p))
+    for call in (opt.step, opt.refresh_images):
+        with pytest.raises(NsrError, match="another `params`"):
+            call()
+    assert torch.equal(p, before) and opt.taken_steps() == 1
+    assert torch.equal(net.half_params(net.params), net.params.detach().half())
