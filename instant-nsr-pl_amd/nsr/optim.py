@@ -253,7 +253,9 @@ class AdamW(torch.optim.Optimizer):
         return self._step if self._step_dev is None else int(self._step_dev.item())
 
     def set_step(self, count):
-        """the next step is number ``count`` + 1"""
+        """the next step is number ``count`` + 1 (``count`` >= 0)"""
+        if not 0 <= int(count) < (1 << 31) - 1:
+            raise ValueError(f"AdamW: a step count of {count}")
         self._step = int(count)
         if self._step_dev is not None:
             self._step_dev.fill_(self._step)

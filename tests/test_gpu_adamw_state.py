@@ -267,3 +267,17 @@ def test_a_module_with_another_parameter_is_refused():
             call()
     assert torch.equal(p, before) and opt.taken_steps() == 1
     assert torch.equal(net.half_params(net.params), net.params.detach().half())
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_step_counts_that_are_none(capturable):
+    """a step number of 0 or less would divide by 1 - beta^0"""
+    new, gs = _pair(300)
+    p, opt = new(capturable=capturable)
+    for bad in (-1, -5, 1 << 31):
+        with pytest.raises(ValueError):
+            opt.set_step(bad)
+    opt.set_step(0)
+    p.grad = gs[0]
+    opt.step()
+    assert opt.taken_steps() == 1 and torch.isfinite(p).all()
