@@ -327,12 +327,12 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         b1, b2, eps = self._shared_hyperparameters()
-        scale, found = getattr(self, "grad_scale", None), getattr(self, "found_inf", None)
-        if self._step_dev is None and (scale is not None or found is not None):
-            self._device_step()  # (a step may be left out: only the device knows the count)
         capturing = torch.cuda.is_current_stream_capturing()
         if capturing and not self._capturable:
             raise NsrError("AdamW: only an optimizer with capturable=True can step inside a graph capture")
+        scale, found = getattr(self, "grad_scale", None), getattr(self, "found_inf", None)
+        if self._step_dev is None and (scale is not None or found is not None):
+            self._device_step()  # (a step may be left out: only the device knows the count)
         f = self._fields
         rates = [self._learning_rate(g) for g in self.param_groups]
         if len(rates) == 1:

@@ -281,3 +281,21 @@ def test_step_counts_that_are_none(capturable):
     p.grad = gs[0]
     opt.step()
     assert opt.taken_steps() == 1 and torch.isfinite(p).all()
+
+
+def test_a_refused_captured_step_leaves_the_step_count_alone():
+    """with a GradScaler's scalars: the refusal comes before the step count would be made inside the capture"""
+    from nsr_hip import NsrError
+    new, gs = _pair(300)
+    (p, opt), (q, ref) = new(), new()
+    for o in (opt, ref):
+        o.found_inf, o.grad_scale = torch.zeros(1, device="cuda"), torch.full((1,), 2.0, device="cuda")
+    p.grad = q.grad = gs[0]
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(NsrError):
+        with torch.cuda.graph(graph):
+            opt.step()
+    assert opt.taken_steps() == 0
+    for o in (opt, ref):
+        o.step()
+    assert torch.equal(p, q) and opt.taken_steps() == ref.taken_steps() == 1
