@@ -1091,10 +1091,11 @@ int nsr_adamw_begin_clipped(const NsrAdamwTensor *tensors, uint32_t n_tensors, d
                             const float *found_inf, void *stream);
 
 /* ------------------------------------------------------------------------------------------------
- * Layer norm over the last axis, for networks beside the fused 64-wide ones (the reference's VanillaMLP takes any torch layer:
- * models/network_utils.py:100-139).  Types as above; weight and bias (both may be NULL) are fp32 or of the input's type.
+ * Layer norm over the last axis, for networks that a user builds from torch layers beside the fused 64-wide ones.  (No network of
+ * the reference normalises: its VanillaMLP is linear layers and an activation, models/network_utils.py:100-139.)  Types as above;
+ * weight and bias (both may be NULL) are fp32 or of the input's type.
  * x and dy have a row stride in elements (of a single row it is not looked at), y and dx are contiguous and overlap no input.
- * Statistics and sums in fp32.
+ * Statistics and sums in fp32; the mean is good to its last place also where it is far above the rows' spread.
  * ------------------------------------------------------------------------------------------------ */
 /* y = (x - mean) * rstd * weight + bias; mean / rstd (float[rows], both or neither) are kept for the backward pass */
 int nsr_layer_norm_forward(const void *x, uint64_t x_stride, const void *weight, const void *bias, void *y, float *mean,

@@ -452,7 +452,7 @@ __device__ __forceinline__ void store_sum(uint32_t share, uint32_t shares, int w
     }
 }
 
-// Bound by HBM: 262144 x 64 fp32 in 34 us (6.0 TB/s, a part of it cached), 131072 x 256 bf16 in 35 us (5.8 TB/s), 8192 x 4096
+// Bound by HBM: 262144 x 64 fp32 in 34 to 36 us (6.0 TB/s, a part of it cached), 131072 x 256 bf16 in 35 us (5.8 TB/s), 8192 x 4096
 // bf16 in 38 us (5.4 TB/s with the partial sums); the launch that adds those takes 4 to 5 us.  1024 threads a workgroup, one
 // workgroup a CU: halves or quarters of that with as many more workgroups only made more partial sums (both directions of
 // 8192 x 4096 bf16: 69.7 and 76.5 us).  The next row of each group is under way as soon as this one is in fp32 registers.  (Two

@@ -99,6 +99,7 @@ __device__ __forceinline__ void adamw_elem(float &p, float &m, float &v, float g
 }
 
 // ---- random bits and e4m3 ------------------------------------------------------------------------------------------------
+// (steps and constants: the 32-bit finaliser published with MurmurHash3, in the public domain)
 __device__ __forceinline__ uint32_t mix32(uint32_t x)
 {
     x ^= x >> 16;

@@ -1,5 +1,6 @@
-"""Network layers beside the fused 64-wide networks of ``tinycudann``: modules over ``nsr_hip.ops`` for the fp32 / 16-bit heads
-that a user builds from torch layers (the reference's ``VanillaMLP`` is such a stack: models/network_utils.py:100-139)."""
+"""Network layers beside the fused 64-wide networks of ``tinycudann``: modules over ``nsr_hip.ops`` for networks that a user builds
+from torch layers.  Nothing in this package uses them (no network of the reference normalises: its ``VanillaMLP`` is linear layers
+and an activation, models/network_utils.py:100-139)."""
 import torch
 import torch.nn as nn
 
