@@ -111,8 +111,10 @@ __device__ __forceinline__ float quotient(float t, float n, float inv_n)
 struct Statistics { float off, rstd; };
 __device__ __forceinline__ Statistics row_statistics(float squares, float sum, float inv_n, float eps)
 {
-    const float off = sum * inv_n, var = fmaf(-off, off, squares * inv_n);
-    return {off, inverse_sqrt((var < 0.f ? 0.f : var) + eps)};  // (under 0 by rounding alone; NaN stays)
+    const float off = sum * inv_n, about = squares * inv_n;
+    // (the difference is under 0 by rounding alone; squares past fp32, where off's may be too, leave 1 / sqrt at 0, and NaN stays)
+    const float var = about < __builtin_inff() ? fmaxf(fmaf(-off, off, about), 0.f) : about;
+    return {off, inverse_sqrt(var + eps)};
 }
 
 // sum of f(k) g(k), k < N, in two chains of fma

@@ -87,3 +87,25 @@ def test_mean_far_above_the_spread(dtype, width, offset):
                  + _store(want, dtype)).all())
     assert bool(((mean.double() - m64[:, 0]).abs() <= (E + U * m64.abs())[:, 0]).all())
     assert bool(((rstd.double() / s[:, 0] - 1).abs() <= rel[:, 0] + 4 * U).all())
+
+
+@pytest.mark.parametrize("width", WIDTHS)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_squares_past_fp32_and_values_that_are_none(dtype, width):
+    """rows whose squares overflow fp32 have a reciprocal deviation of 0, as the sum in fp32 says: y is the bias, nothing is NaN.
+    A NaN or an infinity makes its own row NaN and no other"""
+    from nsr_hip import ops
+    g = torch.Generator(device="cuda").manual_seed(width)
+    w, b, _ = _affine(width, 2)
+    x = torch.randn(9, width, generator=g, device="cuda")
+    clean = ops.layer_norm_forward(x.to(dtype), w, b)
+    for k, scale in ((1, 1e21), (3, 1e25), (5, 1e30)):
+        x[k] = scale * (1 + torch.rand(width, generator=g, device="cuda"))
+        x[k, 0] = -scale
+    x[6, width // 2], x[7, width - 1] = float("nan"), float("inf")
+    y, mean, rstd = ops.layer_norm_forward(x.to(dtype), w, b)
+    for k in (1, 3, 5):
+        assert torch.equal(y[k], b.to(dtype)) and float(rstd[k]) == 0.0 and torch.isfinite(mean[k])
+    assert torch.isnan(y[6]).all() and torch.isnan(y[7]).all() and torch.isnan(mean[6]) and torch.isnan(rstd[6:8]).all()
+    rest = [0, 2, 4, 8]
+    assert all(torch.equal(p[rest], q[rest]) for p, q in zip((y, mean, rstd), clean))
